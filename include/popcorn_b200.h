@@ -121,6 +121,41 @@ int b200_add_rms_norm_backward(const void* grad_y, const void* grad_s, const voi
                                void* stream);
 
 /*
+ * The norm that joins a block to the residual stream (x: the block's output), in fp32 from the inputs to one rounding of
+ * each output:
+ *   n = x r1 (post_weight + offset),  r1 = 1 / sqrt(mean(x^2) + eps)     (n = x if post_weight is NULL)
+ *   s = residual_scale * residual + scale * act(gate) * n                (act(gate) = 1 if gate is NULL)
+ *   y = s r2 (weight + offset),       r2 = 1 / sqrt(mean(s^2) + eps)     (of the unrounded s)
+ * act: activation 0 identity, 1 tanh, 2 sigmoid.  gate: [gate_rows, cols], rows / gate_rows consecutive rows share a gate
+ * row (1: a gate per channel; rows: one of its own for each row).  y and s: the normalised input of the next block and
+ * the new residual stream; neither may alias an input.  stats: fp32 [rows][2] = (r1, r2) for the backward, or NULL
+ * (r1 is 1 without post_weight).
+ *
+ * Extends add_rms_norm (src/popcorn/kernels/add_rms_norm.py:8-23), which popcorn has without the norm after the block,
+ * the gate and the scales.
+ */
+int b200_gated_add_rms_norm(const void* x, const void* residual, const void* weight, const void* post_weight, const void* gate,
+                            void* y, void* s, float* stats, int64_t rows, int64_t cols, int64_t gate_rows,
+                            int64_t ldx, int64_t ldr, int64_t ldgate, int64_t ldy, int64_t lds,
+                            int dtype, int activation, double scale, double residual_scale, double eps, double offset, void* stream);
+
+/*
+ * Backward of b200_gated_add_rms_norm from its inputs, its stats and the gradients of y and s (grad_s may be NULL: none).
+ * grad_x, grad_residual: [rows, cols] contiguous; grad_weight, grad_post_weight: [cols]; grad_gate: [gate_rows, cols]
+ * contiguous.  grad_post_weight and grad_gate are NULL exactly where post_weight and gate are.  fp32 throughout, one
+ * rounding of each gradient; sums over rows have a fixed order.  With rows == 0 the parameters' gradients are zeros.
+ * scratch: b200_gated_add_rms_norm_backward_scratch_bytes(rows, cols, gate_rows, dtype) bytes (gate_rows: 0 without a
+ * gate), 16-byte aligned, written by the call.
+ */
+int b200_gated_add_rms_norm_backward_scratch_bytes(int64_t rows, int64_t cols, int64_t gate_rows, int dtype, size_t* bytes);
+int b200_gated_add_rms_norm_backward(const void* grad_y, const void* grad_s, const void* x, const void* residual, const void* weight,
+                                     const void* post_weight, const void* gate, const float* stats, void* grad_x, void* grad_residual,
+                                     void* grad_weight, void* grad_post_weight, void* grad_gate, int64_t rows, int64_t cols,
+                                     int64_t gate_rows, int64_t ldgy, int64_t ldgs, int64_t ldx, int64_t ldr, int64_t ldgate, int dtype,
+                                     int activation, double scale, double residual_scale, double offset, void* scratch,
+                                     size_t scratch_bytes, void* stream);
+
+/*
  * Rotary position embedding over x[batch, seq, heads, head_dim]:
  *   interleaved == 0 (GPT-NeoX halves): (x[j], x[half + j]) rotated by angle (seq, j)
  *   interleaved != 0 (GPT-J pairs):     (x[2j], x[2j + 1])
@@ -344,6 +379,54 @@ int b200_sigmoid_gate_backward(const void* grad_out, const void* a, const void* 
 int b200_moe_route(const void* logits, int32_t* indices, float* weights,
                    int64_t tokens, int64_t experts, int64_t top_k, int64_t ld_logits,
                    int logits_dtype, void* stream);
+
+/*
+ * Balance loss and z-loss of the router, and the picks per expert.  The tokens are [groups, tokens]; groups == 1 takes the
+ * loss over the whole batch, groups == batch sequence by sequence (the mean over the sequences that have a token).  Of the
+ * tokens that the mask keeps (all if mask is NULL, else those whose byte is not 0), n_g in group g, n altogether:
+ *   f_ge = experts * counts_ge / (top_k n_g),  P_ge = sum_t softmax(logits_t)_e / n_g
+ *   *balance = mean over groups with n_g > 0 of sum_e f_ge P_ge       (1 when picks and probabilities are even)
+ *   *z = sum_t logsumexp(logits_t)^2 / n                              (both 0 without a token)
+ * counts: int32 [groups, experts], the kept tokens' picks; one outside [0, experts) is left out.  Masked rows of logits and
+ * indices are not looked at.  A kept row of -inf alone gives NaN, as its softmax does.
+ * logits: [groups * tokens, experts] (ld_logits elements per row); indices: int32 [groups * tokens, top_k], the picks of
+ * b200_moe_route.  stats: fp32 [groups * tokens][2] (row maximum and sum, written for kept rows) or NULL; table: fp32
+ * [groups * (experts + 1) + 1]; the backward reads both.  Limits: experts <= 1024, top_k <= min(experts, 32), groups <=
+ * 65535, fewer than 2^31 picks.  scratch: b200_moe_balance_scratch_bytes() bytes, 16-byte aligned, not to be shared by
+ * calls that may run at the same time.  Sums are fp32 within a CTA and fp64 over the CTAs, in a fixed order.
+ *
+ * popcorn's momoe takes router logits and has no such loss (src/popcorn/kernels/momoe.py:34-53).
+ */
+int b200_moe_balance_scratch_bytes(int64_t groups, int64_t tokens, int64_t experts, size_t* bytes);
+int b200_moe_balance_loss(const void* logits, const int32_t* indices, const uint8_t* mask, float* balance, float* z, int32_t* counts,
+                          float* stats, float* table, int64_t groups, int64_t tokens, int64_t experts, int64_t top_k,
+                          int64_t ld_logits, int logits_dtype, void* scratch, size_t scratch_bytes, void* stream);
+
+/*
+ * grad_logits = *grad_balance * d balance / d logits + *grad_z * d z / d logits (either scalar may be NULL: none; device
+ * memory).  The counts carry no gradient; masked rows get zeros.  logits, mask, stats and table as in the forward call.
+ */
+int b200_moe_balance_loss_backward(const void* logits, const uint8_t* mask, const float* stats, const float* table,
+                                   const float* grad_balance, const float* grad_z, void* grad_logits, int64_t groups, int64_t tokens,
+                                   int64_t experts, int64_t ld_logits, int64_t ld_grad, int logits_dtype, void* stream);
+
+/*
+ * out[t, :] = round_T(scale * weight[ids[t], :]).  ids: int32, or int64 if ids_64 != 0.  An id outside [0, vocab) gives a
+ * row of zeros (a shard of a table is passed with the ids shifted by its first row).  weight: [vocab, cols] with row stride
+ * ldw; cols <= 65535 * 128, tokens <= 2^30, vocab < 2^31.  The row gather of b200_moe_gather with the ids of a batch.
+ */
+int b200_embedding(const void* ids, const void* weight, void* out, int64_t tokens, int64_t vocab, int64_t cols, int64_t ldw,
+                   int64_t ldo, int ids_64, int dtype, double scale, void* stream);
+
+/*
+ * grad_weight[v, :] = round_T(scale * sum over t with ids[t] == v of grad_out[t, :]), fp32, summed in an order that only the
+ * sizes and ids fix; rows without tokens, and the row padding_idx (negative: none), are zeros.  grad_weight: [vocab, cols]
+ * contiguous, every element is written.  scratch: b200_embedding_backward_scratch_bytes() bytes, 16-byte aligned.
+ */
+int b200_embedding_backward_scratch_bytes(int64_t tokens, int64_t vocab, int64_t cols, size_t* bytes);
+int b200_embedding_backward(const void* grad_out, const void* ids, void* grad_weight, int64_t tokens, int64_t vocab, int64_t cols,
+                            int64_t ldg, int64_t padding_idx, int ids_64, int dtype, double scale, void* scratch, size_t scratch_bytes,
+                            void* stream);
 
 /*
  * Bytes of device scratch b200_moe_index needs for this problem size

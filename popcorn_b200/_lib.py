@@ -36,6 +36,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "b200_rms_norm_backward_scratch_bytes": (_int, [_i64, _i64, _int, ctypes.POINTER(_size)]),
     "b200_rms_norm_backward": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _int, _dbl, _ptr, _size, _ptr]),
     "b200_add_rms_norm_backward": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _int, _dbl, _dbl, _ptr, _size, _ptr]),
+    "b200_gated_add_rms_norm": (_int, [_ptr] * 8 + [_i64] * 8 + [_int, _int, _dbl, _dbl, _dbl, _dbl, _ptr]),
+    "b200_gated_add_rms_norm_backward_scratch_bytes": (_int, [_i64, _i64, _i64, _int, ctypes.POINTER(_size)]),
+    "b200_gated_add_rms_norm_backward": (_int, [_ptr] * 13 + [_i64] * 8 + [_int, _int, _dbl, _dbl, _dbl, _ptr, _size, _ptr]),
     "b200_rope": (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _int, _ptr]),
     "b200_rope_qk": (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _int, _ptr]),
     "b200_rope_paired": (_int, [_ptr] * 6 + [_i64] * 18 + [_int, _ptr]),
@@ -55,6 +58,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "b200_geglu_backward": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _ptr]),
     "b200_sigmoid_gate_backward": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _ptr]),
     "b200_moe_route": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _int, _ptr]),
+    "b200_moe_balance_scratch_bytes": (_int, [_i64, _i64, _i64, ctypes.POINTER(_size)]),
+    "b200_moe_balance_loss": (_int, [_ptr] * 8 + [_i64] * 5 + [_int, _ptr, _size, _ptr]),
+    "b200_moe_balance_loss_backward": (_int, [_ptr] * 7 + [_i64] * 5 + [_int, _ptr]),
+    "b200_embedding": (_int, [_ptr] * 3 + [_i64] * 5 + [_int, _int, _dbl, _ptr]),
+    "b200_embedding_backward_scratch_bytes": (_int, [_i64, _i64, _i64, ctypes.POINTER(_size)]),
+    "b200_embedding_backward": (_int, [_ptr] * 3 + [_i64] * 5 + [_int, _int, _dbl, _ptr, _size, _ptr]),
     "b200_moe_index_scratch_bytes": (_int, [_i64, _i64, _i64, ctypes.POINTER(_size)]),
     "b200_moe_index": (_int, [_ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _size, _ptr]),
     "b200_moe_route_index": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _size, _ptr]),

@@ -311,6 +311,66 @@ class _AddRmsNorm(torch.autograd.Function):
         return grad_x, grad_x, grad_w, None, None
 
 
+class _GatedAddRmsNorm(torch.autograd.Function):
+    """Saves the inputs and two numbers per row; the backward forms s again from x and residual, in fp32."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None, gate: Tensor | None, activation: str, scale: float,
+                residual_scale: float, eps: float, offset: float):
+        with torch.no_grad():
+            y, s, stats = ops.gated_add_rms_norm_forward(x, residual, weight, post_weight, gate, activation, scale, residual_scale, eps, offset)
+        ctx.save_for_backward(x, residual, weight, post_weight, gate, stats)
+        ctx.options = (activation, scale, residual_scale, offset)
+        ctx.set_materialize_grads(False)
+        return y, s
+
+    @staticmethod
+    def backward(ctx, grad_y: Tensor | None, grad_s: Tensor | None):
+        x, residual, weight, post_weight, gate, stats = ctx.saved_tensors
+        if grad_y is None and grad_s is None:
+            return (None,) * 10
+        if grad_y is None:  # only the residual stream was used downstream
+            grad_y = torch.zeros_like(grad_s)
+        with torch.no_grad():
+            grads = ops.gated_add_rms_norm_backward(grad_y, grad_s, x, residual, weight, post_weight, gate, stats, *ctx.options)
+        return (*grads, None, None, None, None, None)
+
+
+class _MoeBalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, router_logits: Tensor, indices: Tensor, mask: Tensor | None, per_sequence: bool):
+        with torch.no_grad():
+            balance, z, counts, stats, table = ops.moe_balance_loss_forward(router_logits, indices, mask, per_sequence)
+        ctx.save_for_backward(router_logits, mask, stats, table)
+        ctx.per_sequence = per_sequence
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        return balance, z, counts
+
+    @staticmethod
+    def backward(ctx, grad_balance: Tensor | None, grad_z: Tensor | None, _grad_counts):
+        router_logits, mask, stats, table = ctx.saved_tensors
+        if grad_balance is None and grad_z is None:
+            return None, None, None, None
+        with torch.no_grad():
+            return ops.moe_balance_loss_backward(grad_balance, grad_z, router_logits, mask, stats, table, ctx.per_sequence), None, None, None
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids: Tensor, weight: Tensor, scale: float, padding_idx: int | None) -> Tensor:
+        ctx.save_for_backward(ids)  # the table itself is not needed: an optimizer may already have stepped on it
+        ctx.options = (weight.shape[0], scale, padding_idx)
+        with torch.no_grad():
+            return ops.embedding(ids, weight, scale, padding_idx)
+
+    @staticmethod
+    def backward(ctx, grad_out: Tensor):
+        (ids,) = ctx.saved_tensors
+        with torch.no_grad():
+            return None, ops.embedding_backward(grad_out, ids, *ctx.options), None, None
+
+
 def rms_norm(x: Tensor, weight: Tensor, bias: Tensor | None = None, eps: float = 1e-6) -> Tensor:
     """RMS norm with gradients for x, weight and bias."""
     return _RmsNorm.apply(x, weight, bias, eps)
@@ -381,6 +441,30 @@ def moe_permute(x: Tensor, indices: Tensor, experts: int) -> tuple[Tensor, Tenso
 def moe_unpermute(rows: Tensor, weights: Tensor, pos: Tensor) -> Tensor:
     """Weighted combine with gradients for the expert rows and the gate weights."""
     return _MoeUnpermute.apply(rows, weights, pos)
+
+
+def gated_add_rms_norm(
+    x: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None = None, gate: Tensor | None = None, activation: str = "identity",
+    scale: float = 1.0, residual_scale: float = 1.0, eps: float = 1e-6, offset: float = 0.0,
+) -> tuple[Tensor, Tensor]:
+    """The norms around a block's residual add with gradients for x, residual, both weights and the gate."""
+    if not _needs_grad(x, residual, weight, post_weight, gate):
+        return ops.gated_add_rms_norm(x, residual, weight, post_weight, gate, activation, scale, residual_scale, eps, offset)
+    return _GatedAddRmsNorm.apply(x, residual, weight, post_weight, gate, activation, scale, residual_scale, eps, offset)
+
+
+def moe_balance_loss(router_logits: Tensor, indices: Tensor, mask: Tensor | None = None, per_sequence: bool = False) -> tuple[Tensor, Tensor, Tensor]:
+    """(balance, z, counts) of a router with the gradient of both losses for its logits (the counts carry none)."""
+    if not _needs_grad(router_logits):
+        return ops.moe_balance_loss(router_logits, indices, mask, per_sequence)
+    return _MoeBalanceLoss.apply(router_logits, indices, mask, per_sequence)
+
+
+def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int | None = None) -> Tensor:
+    """Token embedding with a gradient for the table (dense, like the table)."""
+    if not _needs_grad(weight):
+        return ops.embedding(ids, weight, scale, padding_idx)
+    return _Embedding.apply(ids, weight, scale, padding_idx)
 
 
 def _needs_grad(*tensors: Tensor | None) -> bool:

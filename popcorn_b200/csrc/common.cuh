@@ -201,6 +201,15 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
 __device__ __forceinline__ uint4 ld_plain(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 // Read-only 128-bit load that may stay in L1 (weights, cos/sin rows: reused by many warps).
 __device__ __forceinline__ uint4 ld_reuse(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+// A 128-bit load that may stay in L1 and keeps its place behind pdl_prologue().  ld_reuse, like any load through a const
+// __restrict__ pointer, counts as a read of constant data: the compiler may move it above the prologue's wait, where a
+// kernel that this library launched just before may not have written the data yet.  Kernels that read such data at their
+// beginning take their pointers without __restrict__ and load words with this.
+__device__ __forceinline__ uint4 ld_kept(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ void st_stream(void* p, const uint4& v) {
   asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }

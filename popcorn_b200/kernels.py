@@ -72,6 +72,21 @@ def layer_norm(x, weight, bias=None, eps=1e-6):
 
 
 @register_kernel
+def gated_add_rms_norm(x, residual, weight, post_weight=None, gate=None, activation="identity", scale=1.0, residual_scale=1.0, eps=1e-6, offset=0.0):
+    """Norms after a block and before the next, fused with the block's gate and the scaled residual add; returns (y, new residual stream)."""
+
+
+@register_kernel
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """Token embedding: scaled rows of a table."""
+
+
+@register_kernel
+def moe_balance_loss(router_logits, indices, mask=None, per_sequence=False):
+    """Balance loss, z-loss and per-expert counts of a router."""
+
+
+@register_kernel
 def moe_route(router_logits, top_k=2):
     """Softmax over experts, top-k selection, renormalized gate weights."""
 
@@ -97,7 +112,7 @@ def momoe(x, gate_weight, up_weight, down_weight, router_logits, top_k=2):
 
 
 # ops with backward kernels are registered in their differentiable form
-for _op in (rms_norm, add_rms_norm, rms_norm_gated, l2_norm, layer_norm, rotary_embedding, rope, llama4_rope, qk_norm_rope, swiglu, geglu,
+for _op in (rms_norm, add_rms_norm, gated_add_rms_norm, embedding, moe_balance_loss, rms_norm_gated, l2_norm, layer_norm, rotary_embedding, rope, llama4_rope, qk_norm_rope, swiglu, geglu,
             moe_route, moe_permute, moe_unpermute, moe_grouped_gemm, momoe):
     _op.register(BACKEND, source=f"popcorn_b200.autograd.{_op.name}")
 del _op

@@ -21,11 +21,16 @@ Signatures served (names and order are popcorn's):
 and the MoE steps popcorn only has fused inside `momoe`
 (src/popcorn/kernels/momoe.py:47-53, src/popcorn/impls/momoe_tl.py:1071-1161):
   moe_route, moe_index, moe_scatter_rows, moe_permute, moe_gather, moe_unpermute.
+Around the layers, without a counterpart in popcorn:
+  gated_add_rms_norm  the norms after a block and before the next with the block's gate and the residual scale
+  moe_balance_loss    the router's balance loss, z-loss and per-expert counts
+  embedding           the token embedding with its scale
 """
 
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 from torch import Tensor
@@ -63,18 +68,20 @@ def _forbid_grad(*tensors: Tensor | None) -> None:
 
 
 def _rows(t: Tensor) -> tuple[Tensor, int]:
-    """View `t` [..., D] as [rows, D] with a contiguous last dim; returns (view, leading dimension)."""
+    """View `t` [..., D] as [rows, D] with a contiguous last dim; returns (view, leading dimension).  A tensor without such a view, or
+    with rows that overlap (an expanded one), is copied."""
     width = t.shape[-1]
-    if t.dim() == 2 and (t.stride(1) == 1 or width == 1):
-        return t, (t.stride(0) if t.shape[0] > 1 else max(width, 1))
-    if t.dim() >= 1 and (t.stride(-1) == 1 or width == 1):
+    flat = None
+    if t.dim() == 2:
+        flat = t
+    elif t.dim() >= 1 and width and (t.stride(-1) == 1 or width == 1):
         try:
             flat = t.view(-1, width)
         except RuntimeError:
             flat = None
-        if flat is not None and (flat.stride(1) == 1 or width == 1):
-            return flat, (flat.stride(0) if flat.shape[0] > 1 else max(width, 1))
-    flat = t.reshape(-1, width).contiguous()
+    if flat is not None and (flat.stride(1) == 1 or width == 1) and (flat.shape[0] <= 1 or flat.stride(0) >= width):
+        return flat, (flat.stride(0) if flat.shape[0] > 1 else max(width, 1))
+    flat = t.reshape(math.prod(t.shape[:-1]), width).contiguous()
     return flat, max(width, 1)
 
 
@@ -192,6 +199,111 @@ def add_rms_norm_backward(grad_y: Tensor, grad_s: Tensor | None, s: Tensor, weig
                   s2.shape[0], width, ldgy, ldgs, lds, max(width, 1), code, float(eps), float(offset),
                   _ptr(scratch), ctypes.c_size_t(scratch.numel()), _stream(device))
     return grad_x, grad_w
+
+
+ACTIVATIONS = {"identity": 0, "tanh": 1, "sigmoid": 2}  # of the gate, as b200_gated_add_rms_norm numbers them
+
+
+def _gate_rows(x: Tensor, gate: Tensor) -> int:
+    """How many rows of gate values `gate` holds for the rows of x: its leading dimensions are x's up to some dimension and 1 after it."""
+    lead = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape[:-1])
+    count, prefix, fits = 1, True, 1 <= gate.dim() <= x.dim() and gate.shape[-1] == x.shape[-1]
+    for have, want in zip(lead, x.shape[:-1]):
+        prefix = prefix and have == want
+        fits = fits and (prefix or have == 1)
+        count *= have
+    if not fits:
+        raise ValueError(f"gated_add_rms_norm: gate must be [hidden], or have the leading dimensions of x up to some dimension and 1 after it, got {tuple(gate.shape)} for {tuple(x.shape)}")
+    return count
+
+
+def _gated_check(x: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None, gate: Tensor | None, activation: str) -> tuple[torch.device, int, int]:
+    device = _require_cuda(x, residual, weight, post_weight, gate)
+    code = _dtype_code(x, "gated_add_rms_norm")
+    if x.dim() < 1 or residual.shape != x.shape:
+        raise ValueError("gated_add_rms_norm: x must be [..., hidden] and residual of its shape")
+    if weight.shape != x.shape[-1:] or (post_weight is not None and post_weight.shape != x.shape[-1:]):
+        raise ValueError(f"gated_add_rms_norm: weight and post_weight must have shape ({x.shape[-1]},)")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"gated_add_rms_norm: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    for t in (residual, weight, post_weight, gate):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError("gated_add_rms_norm: residual, weights and gate must have the dtype of x")
+    return device, code, 0 if gate is None else _gate_rows(x, gate)
+
+
+def gated_add_rms_norm_forward(
+    x: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None = None, gate: Tensor | None = None, activation: str = "identity",
+    scale: float = 1.0, residual_scale: float = 1.0, eps: float = 1e-6, offset: float = 0.0, want_stats: bool = True,
+) -> tuple[Tensor, Tensor, Tensor | None]:
+    """(y, s, stats) of gated_add_rms_norm; stats (float32 [rows, 2], the reciprocals of both norms' roots) is what its backward takes."""
+    device, code, gate_rows = _gated_check(x, residual, weight, post_weight, gate, activation)
+    _forbid_grad(x, residual, weight, post_weight, gate)
+    width = x.shape[-1]
+    x2, ldx = _rows(x)
+    r2, ldr = _rows(residual)
+    g2, ldgate = (None, 0) if gate is None else _rows(gate)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    s = torch.empty(x.shape, dtype=x.dtype, device=device)
+    stats = torch.empty((x2.shape[0], 2), dtype=torch.float32, device=device) if want_stats else None
+    with torch.cuda.device(device):
+        _lib.call(
+            "b200_gated_add_rms_norm", _ptr(x2), _ptr(r2), _ptr(weight.contiguous()), _ptr(None if post_weight is None else post_weight.contiguous()),
+            _ptr(g2), _ptr(y), _ptr(s), _ptr(stats), x2.shape[0], width, gate_rows, ldx, ldr, ldgate, max(width, 1), max(width, 1), code,
+            ACTIVATIONS[activation], float(scale), float(residual_scale), float(eps), float(offset), _stream(device),
+        )
+    return y, s, stats
+
+
+def gated_add_rms_norm(
+    x: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None = None, gate: Tensor | None = None, activation: str = "identity",
+    scale: float = 1.0, residual_scale: float = 1.0, eps: float = 1e-6, offset: float = 0.0,
+) -> tuple[Tensor, Tensor]:
+    """The norms after a block and before the next, joined to the residual stream in one pass.
+
+    n = rms_norm(x) * (post_weight + offset), or x without post_weight; s = residual_scale * residual + scale *
+    act(gate) * n; returns (rms_norm(s) * (weight + offset), s).  gate: [hidden], or the leading dimensions of x up to
+    some dimension and 1 after it, e.g. [batch, 1, hidden] or the shape of x; activation: identity, tanh or sigmoid.
+    Unlike add_rms_norm nothing is rounded on the way: fp32 from the inputs to one rounding of y and of s."""
+    y, s, _ = gated_add_rms_norm_forward(x, residual, weight, post_weight, gate, activation, scale, residual_scale, eps, offset, want_stats=False)
+    return y, s
+
+
+def gated_add_rms_norm_backward(
+    grad_y: Tensor, grad_s: Tensor | None, x: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None, gate: Tensor | None, stats: Tensor,
+    activation: str = "identity", scale: float = 1.0, residual_scale: float = 1.0, offset: float = 0.0,
+) -> tuple[Tensor, Tensor, Tensor, Tensor | None, Tensor | None]:
+    """(grad_x, grad_residual, grad_weight, grad_post_weight or None, grad_gate or None) of gated_add_rms_norm;
+    `stats` is what gated_add_rms_norm_forward returned for these inputs, grad_s the gradient that arrived for s."""
+    device, code, gate_rows = _gated_check(x, residual, weight, post_weight, gate, activation)
+    _require_cuda(x, grad_y, grad_s, stats)
+    width = x.shape[-1]
+    if grad_y.shape != x.shape or grad_y.dtype != x.dtype or (grad_s is not None and (grad_s.shape != x.shape or grad_s.dtype != x.dtype)):
+        raise ValueError("gated_add_rms_norm_backward: grad_y and grad_s must match x")
+    x2, ldx = _rows(x)
+    rows = x2.shape[0]
+    if stats.shape != (rows, 2) or stats.dtype != torch.float32:
+        raise ValueError("gated_add_rms_norm_backward: stats must be the float32 [rows, 2] of the forward pass")
+    r2, ldr = _rows(residual)
+    gy2, ldgy = _rows(grad_y)
+    gs2, ldgs = (None, 0) if grad_s is None else _rows(grad_s)
+    g2, ldgate = (None, 0) if gate is None else _rows(gate)
+    grad_x = torch.empty(x.shape, dtype=x.dtype, device=device)
+    grad_r = torch.empty(x.shape, dtype=x.dtype, device=device)
+    grad_w = torch.empty(width, dtype=x.dtype, device=device)
+    grad_p = None if post_weight is None else torch.empty(width, dtype=x.dtype, device=device)
+    grad_g = None if gate is None else torch.empty(gate.shape, dtype=x.dtype, device=device)
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(device):
+        _lib.call("b200_gated_add_rms_norm_backward_scratch_bytes", rows, width, gate_rows, code, ctypes.byref(need))
+        scratch = torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
+        _lib.call(
+            "b200_gated_add_rms_norm_backward", _ptr(gy2), _ptr(gs2), _ptr(x2), _ptr(r2), _ptr(weight.contiguous()),
+            _ptr(None if post_weight is None else post_weight.contiguous()), _ptr(g2), _ptr(stats.contiguous()), _ptr(grad_x), _ptr(grad_r), _ptr(grad_w),
+            _ptr(grad_p), _ptr(grad_g), rows, width, gate_rows, ldgy, ldgs, ldx, ldr, ldgate, code, ACTIVATIONS[activation], float(scale),
+            float(residual_scale), float(offset), _ptr(scratch), ctypes.c_size_t(scratch.numel()), _stream(device),
+        )
+    return grad_x, grad_r, grad_w, grad_p, grad_g
 
 
 def _rope_check(x: Tensor, cos: Tensor, sin: Tensor, name: str) -> tuple[int, int]:
@@ -557,6 +669,130 @@ def moe_route(router_logits: Tensor, top_k: int) -> tuple[Tensor, Tensor]:
     with torch.cuda.device(device):
         _lib.call("b200_moe_route", _ptr(logits2), _ptr(indices), _ptr(weights), logits2.shape[0], experts, int(top_k), ld, code, _stream(device))
     return indices, weights
+
+
+def _balance_check(router_logits: Tensor, indices: Tensor, mask: Tensor | None, per_sequence: bool) -> tuple[torch.device, int, int]:
+    device = _require_cuda(router_logits, indices, mask)
+    code = _dtype_code(router_logits, "moe_balance_loss")
+    if router_logits.dim() < 2 or (per_sequence and router_logits.dim() != 3):
+        raise ValueError("moe_balance_loss: router_logits must be [..., tokens, experts], [batch, seq, experts] for per_sequence")
+    if indices.dim() != router_logits.dim() or indices.shape[:-1] != router_logits.shape[:-1] or indices.dtype != torch.int32:
+        raise ValueError("moe_balance_loss: indices must be int32 [..., top_k] over the tokens of router_logits")
+    if mask is not None and (mask.shape != router_logits.shape[:-1] or mask.dtype != torch.bool):
+        raise ValueError("moe_balance_loss: mask must be bool over the tokens of router_logits (True: the token counts)")
+    return device, code, router_logits.shape[0] if per_sequence else 1
+
+
+def moe_balance_loss_forward(
+    router_logits: Tensor, indices: Tensor, mask: Tensor | None = None, per_sequence: bool = False, want_stats: bool = True
+) -> tuple[Tensor, Tensor, Tensor, Tensor | None, Tensor]:
+    """(balance, z, counts, stats, table) of moe_balance_loss; stats and table are what its backward takes."""
+    device, code, groups = _balance_check(router_logits, indices, mask, per_sequence)
+    _forbid_grad(router_logits)
+    experts, top_k = router_logits.shape[-1], indices.shape[-1]
+    logits2, ld = _rows(router_logits)
+    total = logits2.shape[0]
+    tokens = total // groups if groups else 0
+    balance = torch.empty((), dtype=torch.float32, device=device)
+    z = torch.empty((), dtype=torch.float32, device=device)
+    counts = torch.empty((groups, experts) if per_sequence else experts, dtype=torch.int32, device=device)
+    stats = torch.empty((total, 2), dtype=torch.float32, device=device) if want_stats else None
+    table = torch.empty(groups * (experts + 1) + 1, dtype=torch.float32, device=device)
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(device):
+        _lib.call("b200_moe_balance_scratch_bytes", groups, tokens, experts, ctypes.byref(need))
+        scratch = torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
+        _lib.call(
+            "b200_moe_balance_loss", _ptr(logits2), _ptr(indices.contiguous()), _ptr(None if mask is None else mask.contiguous()), _ptr(balance), _ptr(z),
+            _ptr(counts), _ptr(stats), _ptr(table), groups, tokens, experts, top_k, ld, code, _ptr(scratch), ctypes.c_size_t(scratch.numel()), _stream(device),
+        )
+    return balance, z, counts, stats, table
+
+
+def moe_balance_loss(router_logits: Tensor, indices: Tensor, mask: Tensor | None = None, per_sequence: bool = False) -> tuple[Tensor, Tensor, Tensor]:
+    """Balance loss, z-loss and per-expert counts of a router, from its logits and the picks of moe_route.
+
+    router_logits: [..., experts]; indices: int32 [..., top_k]; mask: bool [...], True where the token counts (a padded
+    batch).  balance = sum_e f_e P_e with f_e the share of picks times experts and P_e the mean probability, 1 for an even
+    router; with per_sequence (logits [batch, seq, experts]) the mean of the sequences' own losses, empty ones left out.
+    z = mean(logsumexp^2).  Both are float32 scalars, 0 without tokens; counts: int32 [experts], or [batch, experts]."""
+    return moe_balance_loss_forward(router_logits, indices, mask, per_sequence, want_stats=False)[:3]
+
+
+def moe_balance_loss_backward(
+    grad_balance: Tensor | None, grad_z: Tensor | None, router_logits: Tensor, mask: Tensor | None, stats: Tensor, table: Tensor, per_sequence: bool = False
+) -> Tensor:
+    """Gradient of moe_balance_loss with respect to router_logits from the gradients of its two losses (float32 scalars on the device,
+    either may be None); stats and table are what moe_balance_loss_forward returned."""
+    device = _require_cuda(router_logits, grad_balance, grad_z, mask, stats, table)
+    code = _dtype_code(router_logits, "moe_balance_loss_backward")
+    experts = router_logits.shape[-1]
+    groups = router_logits.shape[0] if per_sequence else 1
+    logits2, ld = _rows(router_logits)
+    total = logits2.shape[0]
+    for g in (grad_balance, grad_z):
+        if g is not None and (g.numel() != 1 or g.dtype != torch.float32):
+            raise ValueError("moe_balance_loss_backward: the losses' gradients must be float32 scalars")
+    if stats.shape != (total, 2) or table.shape != (groups * (experts + 1) + 1,) or not (stats.dtype == table.dtype == torch.float32):
+        raise ValueError("moe_balance_loss_backward: stats and table must be those of the forward pass")
+    if mask is not None and (mask.shape != router_logits.shape[:-1] or mask.dtype != torch.bool):
+        raise ValueError("moe_balance_loss_backward: mask must be that of the forward pass")
+    grad = torch.empty(router_logits.shape, dtype=router_logits.dtype, device=device)
+    with torch.cuda.device(device):
+        _lib.call(
+            "b200_moe_balance_loss_backward", _ptr(logits2), _ptr(None if mask is None else mask.contiguous()), _ptr(stats.contiguous()), _ptr(table.contiguous()),
+            _ptr(grad_balance), _ptr(grad_z), _ptr(grad), groups, total // groups if groups else 0, experts, ld, max(experts, 1), code, _stream(device),
+        )
+    return grad
+
+
+def _embedding_check(ids: Tensor, vocab: int, padding_idx: int | None) -> int:
+    """The padding row as b200_embedding_backward takes it (-1: none)."""
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("embedding: ids must be int32 or int64")
+    if padding_idx is None:
+        return -1
+    if not -vocab <= padding_idx < vocab:
+        raise ValueError(f"embedding: padding_idx {padding_idx} is outside the {vocab} rows of the table")
+    return padding_idx % vocab
+
+
+def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int | None = None) -> Tensor:
+    """scale * weight[ids], [..., hidden]; one rounding.  An id outside the table gives a row of zeros (a shard of a table takes the
+    ids shifted by its first row); padding_idx names a row that gets no gradient."""
+    device = _require_cuda(ids, weight)
+    _forbid_grad(weight)
+    code = _dtype_code(weight, "embedding")
+    if weight.dim() != 2:
+        raise ValueError("embedding: weight must be [vocab, hidden]")
+    vocab, width = weight.shape
+    _embedding_check(ids, vocab, padding_idx)
+    w2, ldw = _rows(weight)
+    out = torch.empty((*ids.shape, width), dtype=weight.dtype, device=device)
+    with torch.cuda.device(device):
+        _lib.call("b200_embedding", _ptr(ids.contiguous()), _ptr(w2), _ptr(out), ids.numel(), vocab, width, ldw, max(width, 1),
+                  int(ids.dtype == torch.int64), code, float(scale), _stream(device))
+    return out
+
+
+def embedding_backward(grad_out: Tensor, ids: Tensor, vocab: int, scale: float = 1.0, padding_idx: int | None = None) -> Tensor:
+    """Gradient of embedding(ids, weight, scale, padding_idx) with respect to its [vocab, hidden] table: the tokens sorted by id, each
+    row's gradients summed in fp32 in a fixed order, rows without tokens zero."""
+    device = _require_cuda(grad_out, ids)
+    code = _dtype_code(grad_out, "embedding_backward")
+    padding = _embedding_check(ids, vocab, padding_idx)
+    if grad_out.dim() < 1 or grad_out.shape[:-1] != ids.shape:
+        raise ValueError("embedding_backward: grad_out must be [..., hidden] over ids")
+    width = grad_out.shape[-1]
+    g2, ldg = _rows(grad_out)
+    grad = torch.empty((vocab, width), dtype=grad_out.dtype, device=device)
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(device):
+        _lib.call("b200_embedding_backward_scratch_bytes", ids.numel(), vocab, width, ctypes.byref(need))
+        scratch = torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
+        _lib.call("b200_embedding_backward", _ptr(g2), _ptr(ids.contiguous()), _ptr(grad), ids.numel(), vocab, width, ldg, padding, int(ids.dtype == torch.int64),
+                  code, float(scale), _ptr(scratch), ctypes.c_size_t(scratch.numel()), _stream(device))
+    return grad
 
 
 def moe_index(indices: Tensor, experts: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
