@@ -317,8 +317,7 @@ class _GatedAddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None, gate: Tensor | None, activation: str, scale: float,
                 residual_scale: float, eps: float, offset: float):
-        with torch.no_grad():
-            y, s, stats = ops.gated_add_rms_norm_forward(x, residual, weight, post_weight, gate, activation, scale, residual_scale, eps, offset)
+        y, s, stats = ops.gated_add_rms_norm_forward(x, residual, weight, post_weight, gate, activation, scale, residual_scale, eps, offset)
         ctx.save_for_backward(x, residual, weight, post_weight, gate, stats)
         ctx.options = (activation, scale, residual_scale, offset)
         ctx.set_materialize_grads(False)
@@ -339,8 +338,7 @@ class _GatedAddRmsNorm(torch.autograd.Function):
 class _MoeBalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, router_logits: Tensor, indices: Tensor, mask: Tensor | None, per_sequence: bool):
-        with torch.no_grad():
-            balance, z, counts, stats, table = ops.moe_balance_loss_forward(router_logits, indices, mask, per_sequence)
+        balance, z, counts, stats, table = ops.moe_balance_loss_forward(router_logits, indices, mask, per_sequence)
         ctx.save_for_backward(router_logits, mask, stats, table)
         ctx.per_sequence = per_sequence
         ctx.mark_non_differentiable(counts)
@@ -361,8 +359,7 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, ids: Tensor, weight: Tensor, scale: float, padding_idx: int | None) -> Tensor:
         ctx.save_for_backward(ids)  # the table itself is not needed: an optimizer may already have stepped on it
         ctx.options = (weight.shape[0], scale, padding_idx)
-        with torch.no_grad():
-            return ops.embedding(ids, weight, scale, padding_idx)
+        return ops.embedding(ids, weight, scale, padding_idx)
 
     @staticmethod
     def backward(ctx, grad_out: Tensor):

@@ -30,6 +30,7 @@ Around the layers, without a counterpart in popcorn:
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -105,6 +106,49 @@ def _ptr(t: Tensor | None) -> ctypes.c_void_p:
 
 def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+# The operators around the layers are called with few rows too, where the host's part is what a call costs: the helpers below do
+# what those above do with fewer objects (no view of a contiguous tensor, no device guard on the current device, the stream's
+# handle instead of a Stream).  A call of gated_add_rms_norm on eight rows takes 17 us of the host with them, 42 us without.
+
+def _one_device(first: Tensor, *others: Tensor | None) -> int:
+    """The index of the CUDA device that all tensors are on."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        _require_cuda(first, *others)  # says what is wrong
+    return index
+
+
+def _layout(t: Tensor) -> tuple[Tensor, int]:
+    """A tensor whose data pointer is that of the rows of `t` (itself, or a copy as in _rows), and their leading dimension."""
+    return (t, t.shape[-1] or 1) if t.is_contiguous() else _rows(t)
+
+
+def _address(t: Tensor | None) -> int:
+    """The caller keeps `t` in a variable until its kernels are enqueued."""
+    return 0 if t is None else t.data_ptr()
+
+
+def _enqueue(index: int, name: str, *args: object) -> None:
+    """Call an entry point whose last argument is the stream: the current one of the device, made current for the call."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        return _lib.call(name, *args, stream)
+    with torch.cuda.device(index):
+        _lib.call(name, *args, stream)
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(index: int, name: str, *sizes: int) -> int:
+    """What a ..._scratch_bytes entry point says for these sizes on this device."""
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(index):
+        _lib.call(name, *sizes, ctypes.byref(need))
+    return max(need.value, 16)
 
 
 def rms_norm(x: Tensor, weight: Tensor, bias: Tensor | None = None, eps: float = 1e-6) -> Tensor:
@@ -206,6 +250,8 @@ ACTIVATIONS = {"identity": 0, "tanh": 1, "sigmoid": 2}  # of the gate, as b200_g
 
 def _gate_rows(x: Tensor, gate: Tensor) -> int:
     """How many rows of gate values `gate` holds for the rows of x: its leading dimensions are x's up to some dimension and 1 after it."""
+    if gate.shape == x.shape[-1:]:
+        return 1
     lead = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape[:-1])
     count, prefix, fits = 1, True, 1 <= gate.dim() <= x.dim() and gate.shape[-1] == x.shape[-1]
     for have, want in zip(lead, x.shape[:-1]):
@@ -217,19 +263,21 @@ def _gate_rows(x: Tensor, gate: Tensor) -> int:
     return count
 
 
-def _gated_check(x: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None, gate: Tensor | None, activation: str) -> tuple[torch.device, int, int]:
-    device = _require_cuda(x, residual, weight, post_weight, gate)
+def _gated_check(x: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None, gate: Tensor | None, activation: str) -> tuple[int, int, int, int]:
+    """(device index, dtype code, gate rows, activation code)"""
+    index = _one_device(x, residual, weight, post_weight, gate)
+    dtype = x.dtype
     code = _dtype_code(x, "gated_add_rms_norm")
     if x.dim() < 1 or residual.shape != x.shape:
         raise ValueError("gated_add_rms_norm: x must be [..., hidden] and residual of its shape")
     if weight.shape != x.shape[-1:] or (post_weight is not None and post_weight.shape != x.shape[-1:]):
         raise ValueError(f"gated_add_rms_norm: weight and post_weight must have shape ({x.shape[-1]},)")
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"gated_add_rms_norm: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
-    for t in (residual, weight, post_weight, gate):
-        if t is not None and t.dtype != x.dtype:
-            raise TypeError("gated_add_rms_norm: residual, weights and gate must have the dtype of x")
-    return device, code, 0 if gate is None else _gate_rows(x, gate)
+    if residual.dtype != dtype or weight.dtype != dtype or (post_weight is not None and post_weight.dtype != dtype) or (gate is not None and gate.dtype != dtype):
+        raise TypeError("gated_add_rms_norm: residual, weights and gate must have the dtype of x")
+    return index, code, 0 if gate is None else _gate_rows(x, gate), act
 
 
 def gated_add_rms_norm_forward(
@@ -237,21 +285,18 @@ def gated_add_rms_norm_forward(
     scale: float = 1.0, residual_scale: float = 1.0, eps: float = 1e-6, offset: float = 0.0, want_stats: bool = True,
 ) -> tuple[Tensor, Tensor, Tensor | None]:
     """(y, s, stats) of gated_add_rms_norm; stats (float32 [rows, 2], the reciprocals of both norms' roots) is what its backward takes."""
-    device, code, gate_rows = _gated_check(x, residual, weight, post_weight, gate, activation)
+    index, code, gate_rows, act = _gated_check(x, residual, weight, post_weight, gate, activation)
     _forbid_grad(x, residual, weight, post_weight, gate)
     width = x.shape[-1]
-    x2, ldx = _rows(x)
-    r2, ldr = _rows(residual)
-    g2, ldgate = (None, 0) if gate is None else _rows(gate)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    s = torch.empty(x.shape, dtype=x.dtype, device=device)
-    stats = torch.empty((x2.shape[0], 2), dtype=torch.float32, device=device) if want_stats else None
-    with torch.cuda.device(device):
-        _lib.call(
-            "b200_gated_add_rms_norm", _ptr(x2), _ptr(r2), _ptr(weight.contiguous()), _ptr(None if post_weight is None else post_weight.contiguous()),
-            _ptr(g2), _ptr(y), _ptr(s), _ptr(stats), x2.shape[0], width, gate_rows, ldx, ldr, ldgate, max(width, 1), max(width, 1), code,
-            ACTIVATIONS[activation], float(scale), float(residual_scale), float(eps), float(offset), _stream(device),
-        )
+    rows = x.numel() // width if width else math.prod(x.shape[:-1])
+    xl, ldx = _layout(x)
+    rl, ldr = _layout(residual)
+    gl, ldgate = (None, 0) if gate is None else _layout(gate)
+    weight, post_weight = weight.contiguous(), None if post_weight is None else post_weight.contiguous()
+    y, s = x.new_empty(x.shape), x.new_empty(x.shape)
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
+    _enqueue(index, "b200_gated_add_rms_norm", xl.data_ptr(), rl.data_ptr(), weight.data_ptr(), _address(post_weight), _address(gl), y.data_ptr(), s.data_ptr(),
+             _address(stats), rows, width, gate_rows, ldx, ldr, ldgate, width or 1, width or 1, code, act, scale, residual_scale, eps, offset)
     return y, s, stats
 
 
@@ -275,34 +320,27 @@ def gated_add_rms_norm_backward(
 ) -> tuple[Tensor, Tensor, Tensor, Tensor | None, Tensor | None]:
     """(grad_x, grad_residual, grad_weight, grad_post_weight or None, grad_gate or None) of gated_add_rms_norm;
     `stats` is what gated_add_rms_norm_forward returned for these inputs, grad_s the gradient that arrived for s."""
-    device, code, gate_rows = _gated_check(x, residual, weight, post_weight, gate, activation)
-    _require_cuda(x, grad_y, grad_s, stats)
+    index, code, gate_rows, act = _gated_check(x, residual, weight, post_weight, gate, activation)
+    _one_device(x, grad_y, grad_s, stats)
     width = x.shape[-1]
     if grad_y.shape != x.shape or grad_y.dtype != x.dtype or (grad_s is not None and (grad_s.shape != x.shape or grad_s.dtype != x.dtype)):
         raise ValueError("gated_add_rms_norm_backward: grad_y and grad_s must match x")
-    x2, ldx = _rows(x)
-    rows = x2.shape[0]
+    rows = x.numel() // width if width else math.prod(x.shape[:-1])
     if stats.shape != (rows, 2) or stats.dtype != torch.float32:
         raise ValueError("gated_add_rms_norm_backward: stats must be the float32 [rows, 2] of the forward pass")
-    r2, ldr = _rows(residual)
-    gy2, ldgy = _rows(grad_y)
-    gs2, ldgs = (None, 0) if grad_s is None else _rows(grad_s)
-    g2, ldgate = (None, 0) if gate is None else _rows(gate)
-    grad_x = torch.empty(x.shape, dtype=x.dtype, device=device)
-    grad_r = torch.empty(x.shape, dtype=x.dtype, device=device)
-    grad_w = torch.empty(width, dtype=x.dtype, device=device)
-    grad_p = None if post_weight is None else torch.empty(width, dtype=x.dtype, device=device)
-    grad_g = None if gate is None else torch.empty(gate.shape, dtype=x.dtype, device=device)
-    need = ctypes.c_size_t(0)
-    with torch.cuda.device(device):
-        _lib.call("b200_gated_add_rms_norm_backward_scratch_bytes", rows, width, gate_rows, code, ctypes.byref(need))
-        scratch = torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
-        _lib.call(
-            "b200_gated_add_rms_norm_backward", _ptr(gy2), _ptr(gs2), _ptr(x2), _ptr(r2), _ptr(weight.contiguous()),
-            _ptr(None if post_weight is None else post_weight.contiguous()), _ptr(g2), _ptr(stats.contiguous()), _ptr(grad_x), _ptr(grad_r), _ptr(grad_w),
-            _ptr(grad_p), _ptr(grad_g), rows, width, gate_rows, ldgy, ldgs, ldx, ldr, ldgate, code, ACTIVATIONS[activation], float(scale),
-            float(residual_scale), float(offset), _ptr(scratch), ctypes.c_size_t(scratch.numel()), _stream(device),
-        )
+    xl, ldx = _layout(x)
+    rl, ldr = _layout(residual)
+    gyl, ldgy = _layout(grad_y)
+    gsl, ldgs = (None, 0) if grad_s is None else _layout(grad_s)
+    gl, ldgate = (None, 0) if gate is None else _layout(gate)
+    weight, post_weight, stats = weight.contiguous(), None if post_weight is None else post_weight.contiguous(), stats.contiguous()
+    grad_x, grad_r, grad_w = x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(width)
+    grad_p = None if post_weight is None else x.new_empty(width)
+    grad_g = None if gate is None else x.new_empty(gate.shape)
+    scratch = x.new_empty(_scratch_bytes(index, "b200_gated_add_rms_norm_backward_scratch_bytes", rows, width, gate_rows, code), dtype=torch.uint8)
+    _enqueue(index, "b200_gated_add_rms_norm_backward", gyl.data_ptr(), _address(gsl), xl.data_ptr(), rl.data_ptr(), weight.data_ptr(), _address(post_weight), _address(gl),
+             stats.data_ptr(), grad_x.data_ptr(), grad_r.data_ptr(), grad_w.data_ptr(), _address(grad_p), _address(grad_g), rows, width, gate_rows, ldgy, ldgs, ldx, ldr,
+             ldgate, code, act, scale, residual_scale, offset, scratch.data_ptr(), scratch.numel())
     return grad_x, grad_r, grad_w, grad_p, grad_g
 
 
@@ -671,41 +709,39 @@ def moe_route(router_logits: Tensor, top_k: int) -> tuple[Tensor, Tensor]:
     return indices, weights
 
 
-def _balance_check(router_logits: Tensor, indices: Tensor, mask: Tensor | None, per_sequence: bool) -> tuple[torch.device, int, int]:
-    device = _require_cuda(router_logits, indices, mask)
+def _balance_check(router_logits: Tensor, indices: Tensor, mask: Tensor | None, per_sequence: bool) -> tuple[int, int, int]:
+    """(device index, dtype code, groups)"""
+    index = _one_device(router_logits, indices, mask)
     code = _dtype_code(router_logits, "moe_balance_loss")
+    lead = router_logits.shape[:-1]
     if router_logits.dim() < 2 or (per_sequence and router_logits.dim() != 3):
         raise ValueError("moe_balance_loss: router_logits must be [..., tokens, experts], [batch, seq, experts] for per_sequence")
-    if indices.dim() != router_logits.dim() or indices.shape[:-1] != router_logits.shape[:-1] or indices.dtype != torch.int32:
+    if indices.dim() != router_logits.dim() or indices.shape[:-1] != lead or indices.dtype != torch.int32:
         raise ValueError("moe_balance_loss: indices must be int32 [..., top_k] over the tokens of router_logits")
-    if mask is not None and (mask.shape != router_logits.shape[:-1] or mask.dtype != torch.bool):
+    if mask is not None and (mask.shape != lead or mask.dtype != torch.bool):
         raise ValueError("moe_balance_loss: mask must be bool over the tokens of router_logits (True: the token counts)")
-    return device, code, router_logits.shape[0] if per_sequence else 1
+    return index, code, lead[0] if per_sequence else 1
 
 
 def moe_balance_loss_forward(
     router_logits: Tensor, indices: Tensor, mask: Tensor | None = None, per_sequence: bool = False, want_stats: bool = True
 ) -> tuple[Tensor, Tensor, Tensor, Tensor | None, Tensor]:
     """(balance, z, counts, stats, table) of moe_balance_loss; stats and table are what its backward takes."""
-    device, code, groups = _balance_check(router_logits, indices, mask, per_sequence)
+    index, code, groups = _balance_check(router_logits, indices, mask, per_sequence)
     _forbid_grad(router_logits)
     experts, top_k = router_logits.shape[-1], indices.shape[-1]
-    logits2, ld = _rows(router_logits)
-    total = logits2.shape[0]
+    total = math.prod(router_logits.shape[:-1])
     tokens = total // groups if groups else 0
-    balance = torch.empty((), dtype=torch.float32, device=device)
-    z = torch.empty((), dtype=torch.float32, device=device)
-    counts = torch.empty((groups, experts) if per_sequence else experts, dtype=torch.int32, device=device)
-    stats = torch.empty((total, 2), dtype=torch.float32, device=device) if want_stats else None
-    table = torch.empty(groups * (experts + 1) + 1, dtype=torch.float32, device=device)
-    need = ctypes.c_size_t(0)
-    with torch.cuda.device(device):
-        _lib.call("b200_moe_balance_scratch_bytes", groups, tokens, experts, ctypes.byref(need))
-        scratch = torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
-        _lib.call(
-            "b200_moe_balance_loss", _ptr(logits2), _ptr(indices.contiguous()), _ptr(None if mask is None else mask.contiguous()), _ptr(balance), _ptr(z),
-            _ptr(counts), _ptr(stats), _ptr(table), groups, tokens, experts, top_k, ld, code, _ptr(scratch), ctypes.c_size_t(scratch.numel()), _stream(device),
-        )
+    ll, ld = _layout(router_logits)
+    indices, mask = indices.contiguous(), None if mask is None else mask.contiguous()
+    new = router_logits.new_empty
+    balance, z = new((), dtype=torch.float32), new((), dtype=torch.float32)
+    counts = new((groups, experts) if per_sequence else experts, dtype=torch.int32)
+    stats = new((total, 2), dtype=torch.float32) if want_stats else None
+    table = new(groups * (experts + 1) + 1, dtype=torch.float32)
+    scratch = new(_scratch_bytes(index, "b200_moe_balance_scratch_bytes", groups, tokens, experts), dtype=torch.uint8)
+    _enqueue(index, "b200_moe_balance_loss", ll.data_ptr(), indices.data_ptr(), _address(mask), balance.data_ptr(), z.data_ptr(), counts.data_ptr(), _address(stats),
+             table.data_ptr(), groups, tokens, experts, top_k, ld, code, scratch.data_ptr(), scratch.numel())
     return balance, z, counts, stats, table
 
 
@@ -724,12 +760,11 @@ def moe_balance_loss_backward(
 ) -> Tensor:
     """Gradient of moe_balance_loss with respect to router_logits from the gradients of its two losses (float32 scalars on the device,
     either may be None); stats and table are what moe_balance_loss_forward returned."""
-    device = _require_cuda(router_logits, grad_balance, grad_z, mask, stats, table)
+    index = _one_device(router_logits, grad_balance, grad_z, mask, stats, table)
     code = _dtype_code(router_logits, "moe_balance_loss_backward")
     experts = router_logits.shape[-1]
     groups = router_logits.shape[0] if per_sequence else 1
-    logits2, ld = _rows(router_logits)
-    total = logits2.shape[0]
+    total = math.prod(router_logits.shape[:-1])
     for g in (grad_balance, grad_z):
         if g is not None and (g.numel() != 1 or g.dtype != torch.float32):
             raise ValueError("moe_balance_loss_backward: the losses' gradients must be float32 scalars")
@@ -737,12 +772,11 @@ def moe_balance_loss_backward(
         raise ValueError("moe_balance_loss_backward: stats and table must be those of the forward pass")
     if mask is not None and (mask.shape != router_logits.shape[:-1] or mask.dtype != torch.bool):
         raise ValueError("moe_balance_loss_backward: mask must be that of the forward pass")
-    grad = torch.empty(router_logits.shape, dtype=router_logits.dtype, device=device)
-    with torch.cuda.device(device):
-        _lib.call(
-            "b200_moe_balance_loss_backward", _ptr(logits2), _ptr(None if mask is None else mask.contiguous()), _ptr(stats.contiguous()), _ptr(table.contiguous()),
-            _ptr(grad_balance), _ptr(grad_z), _ptr(grad), groups, total // groups if groups else 0, experts, ld, max(experts, 1), code, _stream(device),
-        )
+    ll, ld = _layout(router_logits)
+    mask, stats, table = None if mask is None else mask.contiguous(), stats.contiguous(), table.contiguous()
+    grad = router_logits.new_empty(router_logits.shape)
+    _enqueue(index, "b200_moe_balance_loss_backward", ll.data_ptr(), _address(mask), stats.data_ptr(), table.data_ptr(), _address(grad_balance), _address(grad_z),
+             grad.data_ptr(), groups, total // groups if groups else 0, experts, ld, experts or 1, code)
     return grad
 
 
@@ -760,38 +794,35 @@ def _embedding_check(ids: Tensor, vocab: int, padding_idx: int | None) -> int:
 def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int | None = None) -> Tensor:
     """scale * weight[ids], [..., hidden]; one rounding.  An id outside the table gives a row of zeros (a shard of a table takes the
     ids shifted by its first row); padding_idx names a row that gets no gradient."""
-    device = _require_cuda(ids, weight)
+    index = _one_device(weight, ids)
     _forbid_grad(weight)
     code = _dtype_code(weight, "embedding")
     if weight.dim() != 2:
         raise ValueError("embedding: weight must be [vocab, hidden]")
     vocab, width = weight.shape
     _embedding_check(ids, vocab, padding_idx)
-    w2, ldw = _rows(weight)
-    out = torch.empty((*ids.shape, width), dtype=weight.dtype, device=device)
-    with torch.cuda.device(device):
-        _lib.call("b200_embedding", _ptr(ids.contiguous()), _ptr(w2), _ptr(out), ids.numel(), vocab, width, ldw, max(width, 1),
-                  int(ids.dtype == torch.int64), code, float(scale), _stream(device))
+    wl, ldw = _layout(weight)
+    ids = ids.contiguous()
+    out = weight.new_empty((*ids.shape, width))
+    _enqueue(index, "b200_embedding", ids.data_ptr(), wl.data_ptr(), out.data_ptr(), ids.numel(), vocab, width, ldw, width or 1, ids.dtype == torch.int64, code, scale)
     return out
 
 
 def embedding_backward(grad_out: Tensor, ids: Tensor, vocab: int, scale: float = 1.0, padding_idx: int | None = None) -> Tensor:
     """Gradient of embedding(ids, weight, scale, padding_idx) with respect to its [vocab, hidden] table: the tokens sorted by id, each
     row's gradients summed in fp32 in a fixed order, rows without tokens zero."""
-    device = _require_cuda(grad_out, ids)
+    index = _one_device(grad_out, ids)
     code = _dtype_code(grad_out, "embedding_backward")
     padding = _embedding_check(ids, vocab, padding_idx)
     if grad_out.dim() < 1 or grad_out.shape[:-1] != ids.shape:
         raise ValueError("embedding_backward: grad_out must be [..., hidden] over ids")
-    width = grad_out.shape[-1]
-    g2, ldg = _rows(grad_out)
-    grad = torch.empty((vocab, width), dtype=grad_out.dtype, device=device)
-    need = ctypes.c_size_t(0)
-    with torch.cuda.device(device):
-        _lib.call("b200_embedding_backward_scratch_bytes", ids.numel(), vocab, width, ctypes.byref(need))
-        scratch = torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
-        _lib.call("b200_embedding_backward", _ptr(g2), _ptr(ids.contiguous()), _ptr(grad), ids.numel(), vocab, width, ldg, padding, int(ids.dtype == torch.int64),
-                  code, float(scale), _ptr(scratch), ctypes.c_size_t(scratch.numel()), _stream(device))
+    width, tokens = grad_out.shape[-1], ids.numel()
+    gl, ldg = _layout(grad_out)
+    ids = ids.contiguous()
+    grad = grad_out.new_empty((vocab, width))
+    scratch = grad_out.new_empty(_scratch_bytes(index, "b200_embedding_backward_scratch_bytes", tokens, vocab, width), dtype=torch.uint8)
+    _enqueue(index, "b200_embedding_backward", gl.data_ptr(), ids.data_ptr(), grad.data_ptr(), tokens, vocab, width, ldg, padding, ids.dtype == torch.int64, code, scale,
+             scratch.data_ptr(), scratch.numel())
     return grad
 
 
