@@ -1,0 +1,370 @@
+// Shared by the two directions of the gated residual norm (gated_norm.cu, gated_norm_backward.cu).
+#pragma once
+
+#include <algorithm>
+#include <atomic>
+
+#include "common.cuh"
+#include "tma.cuh"
+
+namespace b200 {
+namespace {
+
+enum Activation { kIdentity = 0, kTanh = 1, kSigmoid = 2 };
+
+// One load: a 128-bit word of T, or one element where width, strides or pointers do not allow words.
+template <typename T, bool VEC>
+struct Word;
+template <typename T>
+struct Word<T, true> {
+  static constexpr int N = Num<T>::kVec;
+  using Raw = uint4;
+  static __device__ __forceinline__ Raw zero() { return make_uint4(0, 0, 0, 0); }
+  static __device__ __forceinline__ Raw load(const T* p) { return ld_stream(p); }
+  static __device__ __forceinline__ Raw load_shared_by_rows(const T* p) { return ld_kept(p); }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[N]) { Num<T>::unpack(r, f); }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[N]) { st_stream(p, Num<T>::pack(f)); }
+};
+template <typename T>
+struct Word<T, false> {
+  static constexpr int N = 1;
+  using Raw = T;
+  static __device__ __forceinline__ Raw zero() { return Num<T>::down(0.f); }
+  static __device__ __forceinline__ Raw load(const T* p) { return *p; }
+  static __device__ __forceinline__ Raw load_shared_by_rows(const T* p) { return *p; }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[1]) { f[0] = Num<T>::up(r); }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { *p = Num<T>::down(f[0]); }
+};
+
+__device__ __forceinline__ float activate(float g, int act) {
+  if (act == kTanh) return tanhf(g);
+  if (act == kSigmoid) return __fdiv_rn(1.f, __fadd_rn(1.f, expf(-g)));
+  return g;
+}
+// d act / d g from the activation's value
+__device__ __forceinline__ float activation_slope(float value, int act) {
+  if (act == kTanh) return __fsub_rn(1.f, __fmul_rn(value, value));
+  if (act == kSigmoid) return __fmul_rn(value, __fsub_rn(1.f, value));
+  return 1.f;
+}
+
+// 1 / sqrt(sum of squares / cols + eps), within two units in the last place (nothing is rounded to T in between)
+__device__ __forceinline__ float inv_rms(float sumsq, float inv_cols, float eps) { return rsqrtf(fmaf(sumsq, inv_cols, eps)); }
+
+// N sums over the TPR threads of a row, TPR a power of two.  Up to a warp: shuffles.  Wider: one barrier of those threads
+// (the CTA's, or a named one where several rows share the CTA); `slot` is shared memory of the row that no thread still
+// reads from an earlier call.
+template <int TPR, int THREADS>
+__device__ __forceinline__ void row_barrier() {
+  if constexpr (TPR <= 32) __syncwarp();
+  else if constexpr (TPR == THREADS) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / TPR), "r"(TPR) : "memory");
+}
+template <int TPR, int THREADS>
+__device__ __forceinline__ float row_sum(float v, float* slot) {
+  v = warp_sum(v);
+  if constexpr (TPR > 32) {
+    constexpr int WARPS = TPR / 32;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) slot[(threadIdx.x % TPR) >> 5] = v;
+    row_barrier<TPR, THREADS>();
+    v = slot[lane & (WARPS - 1)];
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
+  }
+  return v;
+}
+// Four at once: two steps leave each lane with a quarter of the lanes' sum of one value (value 2 (lane / 8 % 2) + lane / 16),
+// so six exchanges do for four sums, where one after the other takes twenty.
+template <int TPR, int THREADS>
+__device__ __forceinline__ void row_sums(float (&v)[4], float (*slot)[16]) {
+  const int lane = threadIdx.x & 31;
+  const bool high = lane & 16, odd = lane & 8;
+  const float v01 = (high ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, high ? v[0] : v[1], 16);
+  const float v23 = (high ? v[3] : v[2]) + __shfl_xor_sync(0xffffffffu, high ? v[2] : v[3], 16);
+  float sum = (odd ? v23 : v01) + __shfl_xor_sync(0xffffffffu, odd ? v01 : v23, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if constexpr (TPR > 32) {
+    constexpr int WARPS = TPR / 32;
+    if ((lane & 7) == 0) slot[(odd ? 2 : 0) + (high ? 1 : 0)][(threadIdx.x % TPR) >> 5] = sum;
+    row_barrier<TPR, THREADS>();
+    const float* mine = slot[(odd ? 2 : 0) + (high ? 1 : 0)];
+    sum = mine[lane & (WARPS < 8 ? WARPS - 1 : 7)];
+    if constexpr (WARPS == 16) sum += mine[8 + (lane & 7)];
+#pragma unroll
+    for (int o = WARPS < 8 ? WARPS / 2 : 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  v[0] = __shfl_sync(0xffffffffu, sum, 0);
+  v[1] = __shfl_sync(0xffffffffu, sum, 16);
+  v[2] = __shfl_sync(0xffffffffu, sum, 8);
+  v[3] = __shfl_sync(0xffffffffu, sum, 24);
+}
+
+// ------------------------------------------------------------------- ring --
+//
+// The rows of a walker in shared memory.  Arrays of rows (x, residual, ...) take turns: row r of array a is copy
+// r * arrays + a, in slot (r * arrays + a) % slots, so any number of slots above `arrays` keeps copies in flight.  The
+// copies of a row complete one barrier, barrier r % rows_ahead.  One thread of the walker issues them; a slot is filled
+// again once the walker is past a barrier behind its last read.
+// Every wait is bounded: when one runs out, the walker stops issuing, its threads fetch what they read of the remaining
+// rows with ordinary loads (the data is the same), and it waits, bounded again, for what is in flight before it leaves.
+// A bulk copy moves multiples of 16 bytes between 16-byte boundaries: of a row that starts or ends elsewhere the ring
+// holds what lies between, [lo, hi) in bytes from the row's start, and the few elements around it are loaded directly.
+constexpr int kMaxSlots = 16;
+constexpr int kMaxArrays = 5;
+
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+template <typename T>
+struct RowArray {
+  const T* base;
+  int64_t ld;
+};
+// A row of one array as a thread reads it
+struct RowView {
+  uint32_t memory;  // shared-memory address of the row's first byte (where it would be, for a row off the boundaries)
+  uint32_t lo, hi;  // unused for rows in words
+  const void* row;
+};
+
+template <typename T, bool VEC, int TPR, int THREADS>
+struct Ring {
+  uint64_t* full;
+  unsigned char* memory;
+  volatile int* broken;
+  RowArray<T> arrays[kMaxArrays];
+  int count, slots, rows_ahead;
+  uint32_t row_bytes, slot_bytes;
+  int64_t next, end;  // copies: the next to be issued, and behind the last row's (issuing thread)
+  uint32_t first_row, put_row;
+  int put_array, put, put_bar;  // put_array of put_row is the next copy, into slot put, for barrier put_bar
+  int take, take_bar;
+  uint32_t phase;
+
+  // memory: slots * slot_bytes of this walker; all threads of the CTA call this
+  __device__ __forceinline__ void start(uint64_t* barriers, unsigned char* mem, int* flag, int n, uint32_t bytes, uint32_t padded, uint32_t first, uint32_t last) {
+    full = barriers, memory = mem, broken = flag;
+    slots = n, row_bytes = bytes, slot_bytes = padded, first_row = put_row = first;
+    rows_ahead = (slots + count - 1) / count;  // a barrier is used again only after the row before was given free
+    next = 0, end = static_cast<int64_t>(last - first) * count;
+    put_array = put = put_bar = take = take_bar = 0, phase = 0;
+    if (threadIdx.x % TPR == 0) {
+      *broken = 0;
+      for (int k = 0; k < rows_ahead; ++k) mbar_init(&full[k], count);
+      mbar_init_fence();
+      issue(slots);
+    }
+    __syncthreads();
+  }
+  // bytes of a row that the ring holds, from the row's start
+  __device__ __forceinline__ void span(const T* row, uint32_t& lo, uint32_t& hi) const {
+    if constexpr (VEC) {
+      lo = 0, hi = row_bytes;
+    } else {
+      const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u;
+      lo = (16u - at) & 15u;
+      hi = at + row_bytes < 16u ? 0u : ((at + row_bytes) & ~15u) - at;
+      if (hi < lo) hi = lo;
+    }
+  }
+  // issuing thread: copies up to, not including, `limit`
+  __device__ __forceinline__ void issue(int64_t limit) {
+    for (; next < limit && next < end; ++next) {
+      const T* row = arrays[put_array].base + put_row * arrays[put_array].ld;
+      uint32_t lo, hi;
+      span(row, lo, hi);
+      mbar_arrive_expect(&full[put_bar], hi - lo);
+      if (hi > lo) bulk_load(memory + put * slot_bytes, reinterpret_cast<const unsigned char*>(row) + lo, hi - lo, &full[put_bar]);
+      if (++put == slots) put = 0;
+      if (++put_array == count) {
+        put_array = 0;
+        ++put_row;
+        if (++put_bar == rows_ahead) put_bar = 0;
+      }
+    }
+  }
+  // the walker is past a barrier behind its last read of the first `rows` rows
+  __device__ __forceinline__ void release(int64_t rows) {
+    if (threadIdx.x % TPR == 0 && *broken == 0) issue(rows * count + slots);
+  }
+  // the next row in turn, row first_row + r: has it landed?
+  __device__ __forceinline__ bool wait() {
+    bool landed = *broken == 0;
+    if (landed && !mbar_wait(&full[take_bar], phase)) {
+      *broken = 1;
+      landed = false;
+    }
+    if (++take_bar == rows_ahead) {
+      take_bar = 0;
+      phase ^= 1;
+    }
+    return landed;
+  }
+  // its arrays one after the other, starting with array 0
+  __device__ __forceinline__ RowView view(int a, uint32_t r, bool landed) {
+    RowView v;
+    const T* row = arrays[a].base + static_cast<int64_t>(first_row + r) * arrays[a].ld;
+    v.memory = smem_addr(memory) + take * slot_bytes;
+    if (++take == slots) take = 0;
+    if constexpr (VEC) {
+      if (!landed)
+        for (uint32_t at = (threadIdx.x % TPR) * 16u; at < row_bytes; at += TPR * 16u) st_shared(v.memory + at, ld_stream(reinterpret_cast<const unsigned char*>(row) + at));
+    } else {
+      span(row, v.lo, v.hi);
+      v.memory -= v.lo;
+      if (!landed) v.lo = v.hi = 0;
+      v.row = row;
+    }
+    return v;
+  }
+  // before the walker's memory is left
+  __device__ __forceinline__ void finish() {
+    if (threadIdx.x % TPR == 0 && *broken != 0) {
+      const int64_t rows = (next + count - 1) / count;
+      for (int64_t r = rows > rows_ahead ? rows - rows_ahead : 0; r < rows; ++r) (void)mbar_wait(&full[r % rows_ahead], static_cast<uint32_t>(r / rows_ahead) & 1u);
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t range_start(uint32_t rows, int walkers, int walker) {
+  return static_cast<uint32_t>(static_cast<uint64_t>(rows) * walker / walkers);
+}
+
+// What a thread loads at a time, as fp32 pairs (two elements per instruction): a 128-bit word, or two neighbouring elements
+// of which the second may lie behind the row.
+template <typename T, bool VEC>
+struct Pairs {
+  static constexpr int P = Num<T>::kVec / 2, N = 2 * P;
+  static __device__ __forceinline__ void unpack(const uint4& raw, Float2x (&out)[P]) {
+    float f[N];
+    Num<T>::unpack(raw, f);
+#pragma unroll
+    for (int j = 0; j < P; ++j) out[j] = pack_f2(f[2 * j], f[2 * j + 1]);
+  }
+  static __device__ __forceinline__ void load(const RowView& v, int w, int, Float2x (&out)[P]) { unpack(ld_shared(v.memory + w * 16), out); }
+  static __device__ __forceinline__ void load_shared_by_rows(const T* row, int w, int, Float2x (&out)[P]) { unpack(ld_kept(row + w * N), out); }
+  static __device__ __forceinline__ void store(T* row, int w, int, const Float2x (&v)[P]) {
+    float f[N];
+#pragma unroll
+    for (int j = 0; j < P; ++j) unpack_f2(v[j], f[2 * j], f[2 * j + 1]);
+    st_stream(row + w * N, Num<T>::pack(f));
+  }
+};
+template <typename T>
+struct Pairs<T, false> {
+  static constexpr int P = 1, N = 2;
+  static __device__ __forceinline__ float element(const RowView& v, uint32_t c) {
+    const uint32_t byte = c * static_cast<uint32_t>(sizeof(T));
+    if (byte < v.lo || byte >= v.hi) return Num<T>::up(static_cast<const T*>(v.row)[c]);
+    if constexpr (sizeof(T) == 4) {
+      float f;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(v.memory + byte) : "memory");
+      return f;
+    } else {
+      uint16_t bits;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(v.memory + byte) : "memory");
+      return Num<T>::up(*reinterpret_cast<const T*>(&bits));
+    }
+  }
+  static __device__ __forceinline__ void load(const RowView& v, int w, int cols, Float2x (&out)[1]) {
+    out[0] = pack_f2(element(v, 2 * w), 2 * w + 1 < cols ? element(v, 2 * w + 1) : 0.f);
+  }
+  static __device__ __forceinline__ void load_shared_by_rows(const T* row, int w, int cols, Float2x (&out)[1]) {
+    out[0] = pack_f2(Num<T>::up(row[2 * w]), 2 * w + 1 < cols ? Num<T>::up(row[2 * w + 1]) : 0.f);
+  }
+  static __device__ __forceinline__ void store(T* row, int w, int cols, const Float2x (&v)[1]) {
+    float lo, hi;
+    unpack_f2(v[0], lo, hi);
+    row[2 * w] = Num<T>::down(lo);
+    if (2 * w + 1 < cols) row[2 * w + 1] = Num<T>::down(hi);
+  }
+};
+__device__ __forceinline__ Float2x both(float v) { return pack_f2(v, v); }
+__device__ __forceinline__ float pair_total(Float2x v) {
+  float lo, hi;
+  unpack_f2(v, lo, hi);
+  return __fadd_rn(lo, hi);
+}
+__device__ __forceinline__ Float2x activate2(Float2x g, int act) {
+  float lo, hi;
+  unpack_f2(g, lo, hi);
+  return pack_f2(activate(lo, act), activate(hi, act));
+}
+
+constexpr int kColumns = 16;  // columns per thread of a walker
+constexpr int kMaxWalk = 512;
+constexpr int kWalkColumns = kMaxWalk * kColumns;
+constexpr uint32_t kWalkRows = 2;  // rows per walker from which the forward pass walks
+constexpr int kMaxRingBytes = 208 * 1024;
+
+// s of one element, for the kernels that go over a row more than once
+template <typename T>
+__device__ __forceinline__ float stream_value(float x, float residual, float factor, float r1, float residual_scale) {
+  return fmaf(r1 * factor, x, residual_scale * residual);
+}
+// scale * act(gate) * (post_weight + offset) of one column
+template <typename T>
+__device__ __forceinline__ float branch_factor(const T* post, const T* gate_row, int64_t c, float offset, float scale, int act) {
+  float f = scale;
+  if (gate_row != nullptr) f *= activate(Num<T>::up(gate_row[c]), act);
+  if (post != nullptr) f *= Num<T>::up(post[c]) + offset;
+  return f;
+}
+
+// The threads of a walker for a row of `cols`, its rows' slots in shared memory, and how many walkers share `rows`.
+struct WalkPlan {
+  int tpr, walkers, ctas, slots;
+  uint32_t slot_bytes;
+  size_t smem;
+};
+WalkPlan plan_walk(int64_t rows, int64_t cols, size_t element, int arrays) {
+  WalkPlan p;
+  p.tpr = 32;
+  while (p.tpr * kColumns < cols) p.tpr *= p.tpr == 32 ? 4 : 2;  // no kernels of 64 threads: half of 128 do as well
+  const int groups = p.tpr < 256 ? 256 / p.tpr : 1, per_sm = p.tpr < 512 ? 2 : 1;
+  const int64_t most = static_cast<int64_t>(sm_count()) * per_sm * groups;
+  p.walkers = static_cast<int>(std::max<int64_t>(1, std::min(rows, most)));
+  p.ctas = static_cast<int>(ceil_div(p.walkers, groups));
+  p.slot_bytes = static_cast<uint32_t>(std::max<int64_t>(1, ceil_div(cols * static_cast<int64_t>(element), 16)) * 16);
+  const size_t budget = (per_sm == 2 ? 100 : 208) * 1024 / groups;
+  p.slots = static_cast<int>(std::min<size_t>(kMaxSlots, budget / p.slot_bytes));
+  p.smem = static_cast<size_t>(p.slots) * p.slot_bytes * groups;
+  if (p.slots < arrays) p.slots = 0;
+  return p;
+}
+
+// Opt in to more than 48 KB of shared memory, once per kernel and device.
+template <auto kernel>
+int allow_smem(const char* name) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return fail(B200_ERR_DEVICE, "%s: no current device", name);
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return B200_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRingBytes) != cudaSuccess)
+    return fail(B200_ERR_LAUNCH, "%s: %s", name, cudaGetErrorString(cudaGetLastError()));
+  done.fetch_or(bit, std::memory_order_release);
+  return B200_OK;
+}
+
+// Sizes and enums that both directions check alike.
+int check_shapes(const char* fn, int64_t rows, int64_t cols, int64_t gate_rows, const void* gate, int dtype, int activation) {
+  if (!dtype_ok(dtype)) return fail(B200_ERR_DTYPE, "%s: unsupported dtype %d", fn, dtype);
+  if (activation < kIdentity || activation > kSigmoid) return fail(B200_ERR_SHAPE, "%s: unknown activation %d", fn, activation);
+  if (rows < 0 || cols < 0 || gate_rows < 0) return fail(B200_ERR_SHAPE, "%s: negative size (rows=%lld, cols=%lld, gate_rows=%lld)", fn, (long long)rows, (long long)cols, (long long)gate_rows);
+  if (rows > 0x7fffffffLL || cols > 0x7fffffffLL) return fail(B200_ERR_SHAPE, "%s: rows=%lld and cols=%lld must be below 2^31", fn, (long long)rows, (long long)cols);
+  if (rows > 0 && gate != nullptr && (gate_rows == 0 || rows % gate_rows != 0))
+    return fail(B200_ERR_SHAPE, "%s: rows=%lld is not a multiple of gate_rows=%lld", fn, (long long)rows, (long long)gate_rows);
+  return B200_OK;
+}
+
+}  // namespace
+}  // namespace b200
