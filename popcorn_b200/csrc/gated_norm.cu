@@ -162,11 +162,11 @@ gated_walk_kernel(const ForwardArgs<T> a, int walkers, int slots, uint32_t slot_
   const int walker = blockIdx.x * GROUPS + group;
   const uint32_t first = walker < walkers ? range_start(a.rows, walkers, walker) : 0, last = walker < walkers ? range_start(a.rows, walkers, walker + 1) : 0;
   Ring<T, VEC, TPR, THREADS> ring;
-  ring.count = ROW_GATE ? 3 : 2;
-  ring.arrays[0] = {a.x, a.ldx};
-  ring.arrays[1] = {a.residual, a.ldr};
-  if (ROW_GATE) ring.arrays[2] = {a.gate, a.ldgate};
-  ring.start(barriers[group], memory + static_cast<size_t>(group) * slots * slot_bytes, &flags[group], slots, static_cast<uint32_t>(cols) * sizeof(T), slot_bytes, first, last);
+  ring.start(barriers[group], memory + static_cast<size_t>(group) * slots * slot_bytes, &flags[group], slots, static_cast<uint32_t>(cols) * sizeof(T), slot_bytes, first, last, ROW_GATE ? 3 : 2,
+             [&](int array, const T*& base, int64_t& ld) {
+               base = array == 0 ? a.x : array == 1 ? a.residual : a.gate;
+               ld = array == 0 ? a.ldx : array == 1 ? a.ldr : a.ldgate;
+             });
   bool ok[ITEMS];
   Float2x factor[ITEMS][P], weight[ITEMS][P];
   const Float2x offset2 = both(a.offset);
@@ -217,8 +217,8 @@ gated_walk_kernel(const ForwardArgs<T> a, int walkers, int slots, uint32_t slot_
       load_factor(gate_row);
     }
     const bool landed = ring.wait();
-    const RowView xv = ring.view(0, row - first, landed), rv = ring.view(1, row - first, landed);
-    const RowView gv = ROW_GATE ? ring.view(2, row - first, landed) : rv;
+    const RowView xv = ring.view(a.x, a.ldx, row, landed), rv = ring.view(a.residual, a.ldr, row, landed);
+    const RowView gv = ROW_GATE ? ring.view(a.gate, a.ldgate, row, landed) : rv;
     float r1 = 1.f;
     if (a.post != nullptr) {
       Float2x squares = both(0.f);

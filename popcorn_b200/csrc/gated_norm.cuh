@@ -105,7 +105,7 @@ __device__ __forceinline__ void row_sums(float (&v)[4], float (*slot)[16]) {
 //
 // The rows of a walker in shared memory.  Arrays of rows (x, residual, ...) take turns: row r of array a is copy
 // r * arrays + a, in slot (r * arrays + a) % slots, so any number of slots above `arrays` keeps copies in flight.  The
-// copies of a row complete one barrier, barrier r % rows_ahead.  One thread of the walker issues them; a slot is filled
+// copies of a row complete one barrier, barrier r % rows_ahead.  A thread for each array issues them; a slot is filled
 // again once the walker is past a barrier behind its last read.
 // Every wait is bounded: when one runs out, the walker stops issuing, its threads fetch what they read of the remaining
 // rows with ordinary loads (the data is the same), and it waits, bounded again, for what is in flight before it leaves.
@@ -123,11 +123,6 @@ __device__ __forceinline__ void st_shared(uint32_t at, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-template <typename T>
-struct RowArray {
-  const T* base;
-  int64_t ld;
-};
 // A row of one array as a thread reads it
 struct RowView {
   uint32_t memory;  // shared-memory address of the row's first byte (where it would be, for a row off the boundaries)
@@ -137,32 +132,35 @@ struct RowView {
 
 template <typename T, bool VEC, int TPR, int THREADS>
 struct Ring {
-  uint64_t* full;
-  unsigned char* memory;
+  uint32_t full, memory;  // shared-memory addresses
   volatile int* broken;
-  RowArray<T> arrays[kMaxArrays];
   int count, slots, rows_ahead;
   uint32_t row_bytes, slot_bytes;
-  int64_t next, end;  // copies: the next to be issued, and behind the last row's (issuing thread)
-  uint32_t first_row, put_row;
-  int put_array, put, put_bar;  // put_array of put_row is the next copy, into slot put, for barrier put_bar
+  // the issuing threads (the first `count` of the walker, one array each): their array and the next row of it
+  const T* base;
+  int64_t ld;
+  uint32_t put_row, first_row, last_row;
+  int64_t put_copy;  // of the next row of this array
+  int put, put_bar;  // its slot and barrier
   int take, take_bar;
   uint32_t phase;
 
-  // memory: slots * slot_bytes of this walker; all threads of the CTA call this
-  __device__ __forceinline__ void start(uint64_t* barriers, unsigned char* mem, int* flag, int n, uint32_t bytes, uint32_t padded, uint32_t first, uint32_t last) {
-    full = barriers, memory = mem, broken = flag;
-    slots = n, row_bytes = bytes, slot_bytes = padded, first_row = put_row = first;
+  // memory: slots * slot_bytes of this walker; all threads of the CTA call this.  array(a, base, ld) names the rows of array a.
+  template <typename Arrays>
+  __device__ __forceinline__ void start(uint64_t* barriers, unsigned char* mem, int* flag, int n, uint32_t bytes, uint32_t padded, uint32_t first, uint32_t last, int arrays, Arrays&& array) {
+    full = smem_addr(barriers), memory = smem_addr(mem), broken = flag;
+    count = arrays, slots = n, row_bytes = bytes, slot_bytes = padded, put_row = first_row = first, last_row = last;
     rows_ahead = (slots + count - 1) / count;  // a barrier is used again only after the row before was given free
-    next = 0, end = static_cast<int64_t>(last - first) * count;
-    put_array = put = put_bar = take = take_bar = 0, phase = 0;
+    put_copy = put = threadIdx.x % TPR;
+    put_bar = take = take_bar = 0, phase = 0;
+    array(static_cast<int>(put_copy), base, ld);
     if (threadIdx.x % TPR == 0) {
       *broken = 0;
-      for (int k = 0; k < rows_ahead; ++k) mbar_init(&full[k], count);
+      for (int k = 0; k < rows_ahead; ++k) mbar_init(barriers + k, count);
       mbar_init_fence();
-      issue(slots);
     }
     __syncthreads();
+    if (threadIdx.x % TPR < count) issue(slots);
   }
   // bytes of a row that the ring holds, from the row's start
   __device__ __forceinline__ void span(const T* row, uint32_t& lo, uint32_t& hi) const {
@@ -175,30 +173,46 @@ struct Ring {
       if (hi < lo) hi = lo;
     }
   }
-  // issuing thread: copies up to, not including, `limit`
+  // an issuing thread: its array's copies below `limit`
   __device__ __forceinline__ void issue(int64_t limit) {
-    for (; next < limit && next < end; ++next) {
-      const T* row = arrays[put_array].base + put_row * arrays[put_array].ld;
+    for (; put_copy < limit && put_row < last_row; put_copy += count, ++put_row) {
+      const T* row = base + put_row * ld;
       uint32_t lo, hi;
       span(row, lo, hi);
-      mbar_arrive_expect(&full[put_bar], hi - lo);
-      if (hi > lo) bulk_load(memory + put * slot_bytes, reinterpret_cast<const unsigned char*>(row) + lo, hi - lo, &full[put_bar]);
-      if (++put == slots) put = 0;
-      if (++put_array == count) {
-        put_array = 0;
-        ++put_row;
-        if (++put_bar == rows_ahead) put_bar = 0;
-      }
+      const uint32_t bar = full + put_bar * 8;
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(hi - lo) : "memory");
+      if (hi > lo)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(memory + put * slot_bytes),
+                     "l"(reinterpret_cast<const unsigned char*>(row) + lo), "r"(hi - lo), "r"(bar)
+                     : "memory");
+      put += count;
+      if (put >= slots) put -= slots;
+      if (++put_bar == rows_ahead) put_bar = 0;
     }
   }
   // the walker is past a barrier behind its last read of the first `rows` rows
-  __device__ __forceinline__ void release(int64_t rows) {
-    if (threadIdx.x % TPR == 0 && *broken == 0) issue(rows * count + slots);
+  __device__ __forceinline__ void release(uint32_t rows) {
+    if (threadIdx.x % TPR < count && *broken == 0) issue(static_cast<int64_t>(rows) * count + slots);
   }
-  // the next row in turn, row first_row + r: has it landed?
+  static __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+      uint32_t done;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(bar), "r"(parity)
+          : "memory");
+      if (done) return true;
+    }
+    atomicAdd(&g_wait_timeouts, 1u);
+    return false;
+  }
+  // the next row in turn: has it landed?
   __device__ __forceinline__ bool wait() {
     bool landed = *broken == 0;
-    if (landed && !mbar_wait(&full[take_bar], phase)) {
+    if (landed && !wait_for(full + take_bar * 8, phase)) {
       *broken = 1;
       landed = false;
     }
@@ -208,28 +222,29 @@ struct Ring {
     }
     return landed;
   }
-  // its arrays one after the other, starting with array 0
-  __device__ __forceinline__ RowView view(int a, uint32_t r, bool landed) {
+  // its arrays one after the other, starting with array 0: row `row` of the array at `from`
+  __device__ __forceinline__ RowView view(const T* from, int64_t stride, uint32_t row, bool landed) {
     RowView v;
-    const T* row = arrays[a].base + static_cast<int64_t>(first_row + r) * arrays[a].ld;
-    v.memory = smem_addr(memory) + take * slot_bytes;
+    v.memory = memory + take * slot_bytes;
     if (++take == slots) take = 0;
     if constexpr (VEC) {
-      if (!landed)
-        for (uint32_t at = (threadIdx.x % TPR) * 16u; at < row_bytes; at += TPR * 16u) st_shared(v.memory + at, ld_stream(reinterpret_cast<const unsigned char*>(row) + at));
+      if (!landed) {
+        const unsigned char* bytes = reinterpret_cast<const unsigned char*>(from + row * stride);
+        for (uint32_t at = (threadIdx.x % TPR) * 16u; at < row_bytes; at += TPR * 16u) st_shared(v.memory + at, ld_stream(bytes + at));
+      }
     } else {
-      span(row, v.lo, v.hi);
+      v.row = from + row * stride;
+      span(from + row * stride, v.lo, v.hi);
       v.memory -= v.lo;
       if (!landed) v.lo = v.hi = 0;
-      v.row = row;
     }
     return v;
   }
   // before the walker's memory is left
   __device__ __forceinline__ void finish() {
     if (threadIdx.x % TPR == 0 && *broken != 0) {
-      const int64_t rows = (next + count - 1) / count;
-      for (int64_t r = rows > rows_ahead ? rows - rows_ahead : 0; r < rows; ++r) (void)mbar_wait(&full[r % rows_ahead], static_cast<uint32_t>(r / rows_ahead) & 1u);
+      const uint32_t rows = put_row - first_row;
+      for (uint32_t r = rows > static_cast<uint32_t>(rows_ahead) ? rows - rows_ahead : 0; r < rows; ++r) (void)wait_for(full + r % rows_ahead * 8, r / rows_ahead & 1u);
     }
   }
 };

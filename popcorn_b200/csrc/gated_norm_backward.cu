@@ -85,13 +85,12 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
   const int walker = blockIdx.x * GROUPS + group;
   const uint32_t first = walker < a.walkers ? range_start(a.rows, a.walkers, walker) : 0, last = walker < a.walkers ? range_start(a.rows, a.walkers, walker + 1) : 0;
   Ring<T, VEC, TPR, THREADS> ring;
-  ring.count = 0;
-  ring.arrays[ring.count++] = {a.x, a.ldx};
-  ring.arrays[ring.count++] = {a.residual, a.ldr};
-  ring.arrays[ring.count++] = {a.gy, a.ldgy};
-  if (ROW_GATE) ring.arrays[ring.count++] = {a.gate, a.ldgate};
-  if (a.gs != nullptr) ring.arrays[ring.count++] = {a.gs, a.ldgs};
-  ring.start(barriers[group], memory + static_cast<size_t>(group) * slots * slot_bytes, &flags[group], slots, static_cast<uint32_t>(cols) * sizeof(T), slot_bytes, first, last);
+  const bool has_gs = a.gs != nullptr;
+  ring.start(barriers[group], memory + static_cast<size_t>(group) * slots * slot_bytes, &flags[group], slots, static_cast<uint32_t>(cols) * sizeof(T), slot_bytes, first, last, 3 + (ROW_GATE ? 1 : 0) + (has_gs ? 1 : 0),
+             [&](int array, const T*& base, int64_t& ld) {
+               base = array == 0 ? a.x : array == 1 ? a.residual : array == 2 ? a.gy : ROW_GATE && array == 3 ? a.gate : a.gs;
+               ld = array == 0 ? a.ldx : array == 1 ? a.ldr : array == 2 ? a.ldgy : ROW_GATE && array == 3 ? a.ldgate : a.ldgs;
+             });
   bool ok[ITEMS];
   Float2x factor[ITEMS][P], weight[ITEMS][P], sum_w[ITEMS][P], sum_k[ITEMS][P];
   const Float2x offset2 = both(a.offset);
@@ -150,7 +149,6 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
   load_factor(gate_row);
   const Float2x residual_scale2 = both(a.residual_scale), scale2 = both(a.scale);
   const bool tight = slots < 2 * ring.count;  // the next row's copies need slots of this one: a barrier of their own at its end
-  const bool has_gs = a.gs != nullptr;
   float2 stat = first < last ? a.stats[first] : make_float2(0.f, 0.f);  // of the next row: its latency is that of a row
   int parity = 0;
   for (uint32_t row = first; row < last; ++row, parity ^= 1) {
@@ -166,10 +164,9 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
     }
     const float r1 = stat.x, r2 = stat.y;
     if (row + 1 < last) stat = a.stats[row + 1];
-    const uint32_t r = row - first;
     const bool landed = ring.wait();
-    const RowView xv = ring.view(0, r, landed), rv = ring.view(1, r, landed), gyv = ring.view(2, r, landed);
-    const RowView gv = ROW_GATE ? ring.view(3, r, landed) : gyv, gsv = has_gs ? ring.view(ROW_GATE ? 4 : 3, r, landed) : gyv;
+    const RowView xv = ring.view(a.x, a.ldx, row, landed), rv = ring.view(a.residual, a.ldr, row, landed), gyv = ring.view(a.gy, a.ldgy, row, landed);
+    const RowView gv = ROW_GATE ? ring.view(a.gate, a.ldgate, row, landed) : gyv, gsv = has_gs ? ring.view(a.gs, a.ldgs, row, landed) : gyv;
     const Float2x r12 = both(r1), r22 = both(r2);
     Float2x value[ROW_GATE ? ITEMS : 1][P];  // of the row's own gate
     Float2x acc[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
