@@ -29,7 +29,6 @@ int sm_count();
 unsigned int rope_wait_timeouts();
 unsigned int norm_wait_timeouts();
 unsigned int gemm_wait_timeouts();
-unsigned int gated_norm_wait_timeouts();
 unsigned int gated_backward_wait_timeouts();
 // rms_norm / add_rms_norm backward through the row-bucket kernel of norm_family.cu (rows of at most 1024 128-bit
 // words held in registers; narrow rows several per warp).  gs: the gradient that arrived for the sum s of

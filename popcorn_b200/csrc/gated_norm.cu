@@ -23,8 +23,7 @@ struct ForwardArgs {
   T *y, *s;
   float2* stats;
   uint32_t rows, period;  // period: consecutive rows that share a gate row
-  int words;              // loads per row of the one-row kernel
-  int columns;
+  int words;              // loads per row
   int64_t ldx, ldr, ldgate, ldy, lds;
   float inv_cols, eps, offset, scale, residual_scale;
   int act;
@@ -87,7 +86,7 @@ gated_add_rms_kernel(const ForwardArgs<T> a) {
       float g[N];
       W::unpack(W::load_shared_by_rows(gr + c), g);
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[j] *= activate(g[j], a.act);
+      for (int j = 0; j < N; ++j) f[j] *= activate<T>(g[j], a.act);
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -144,137 +143,6 @@ gated_add_rms_wide_kernel(const ForwardArgs<T> a, int64_t cols) {
   }
 }
 
-// Many rows: walkers over contiguous ranges, the rows through a ring.  The factor scale act(gate) (post_weight + offset)
-// of a thread's columns stays in registers while rows share it.
-template <typename T, bool VEC, int TPR, bool ROW_GATE>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 2 : 1)
-gated_walk_kernel(const ForwardArgs<T> a, int walkers, int slots, uint32_t slot_bytes) {
-  using PW = Pairs<T, VEC>;
-  constexpr int N = PW::N, P = PW::P, ITEMS = kColumns / N;
-  constexpr int THREADS = TPR < 256 ? 256 : TPR, GROUPS = THREADS / TPR;
-  const int cols = a.columns, words = (cols + N - 1) / N;
-  extern __shared__ __align__(128) unsigned char memory[];
-  __shared__ uint64_t barriers[GROUPS][kMaxSlots];
-  __shared__ int flags[GROUPS];
-  __shared__ float sums_store[GROUPS][2][2][16];
-  pdl_prologue();
-  const int group = threadIdx.x / TPR, lane_in_row = threadIdx.x % TPR;
-  const int walker = blockIdx.x * GROUPS + group;
-  const uint32_t first = walker < walkers ? range_start(a.rows, walkers, walker) : 0, last = walker < walkers ? range_start(a.rows, walkers, walker + 1) : 0;
-  Ring<T, VEC, TPR, THREADS> ring;
-  ring.start(barriers[group], memory + static_cast<size_t>(group) * slots * slot_bytes, &flags[group], slots, static_cast<uint32_t>(cols) * sizeof(T), slot_bytes, first, last, ROW_GATE ? 3 : 2,
-             [&](int array, const T*& base, int64_t& ld) {
-               base = array == 0 ? a.x : array == 1 ? a.residual : a.gate;
-               ld = array == 0 ? a.ldx : array == 1 ? a.ldr : a.ldgate;
-             });
-  bool ok[ITEMS];
-  Float2x factor[ITEMS][P], weight[ITEMS][P];
-  const Float2x offset2 = both(a.offset);
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int w = lane_in_row + i * TPR;
-    ok[i] = w < words;
-#pragma unroll
-    for (int j = 0; j < P; ++j) weight[i][j] = both(0.f);
-    if (ok[i]) {
-      PW::load_shared_by_rows(a.weight, w, cols, weight[i]);
-#pragma unroll
-      for (int j = 0; j < P; ++j) weight[i][j] = add_f2(weight[i][j], offset2);
-    }
-  }
-  auto load_factor = [&](uint32_t gate_row) {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int w = lane_in_row + i * TPR;
-#pragma unroll
-      for (int j = 0; j < P; ++j) factor[i][j] = both(a.scale);
-      if (!ok[i]) continue;
-      Float2x v[P];
-      if (a.post != nullptr) {
-        PW::load_shared_by_rows(a.post, w, cols, v);
-#pragma unroll
-        for (int j = 0; j < P; ++j) factor[i][j] = mul_f2(factor[i][j], add_f2(v[j], offset2));
-      }
-      if (!ROW_GATE && a.gate != nullptr) {
-        PW::load_shared_by_rows(a.gate + static_cast<int64_t>(gate_row) * a.ldgate, w, cols, v);
-#pragma unroll
-        for (int j = 0; j < P; ++j) factor[i][j] = mul_f2(factor[i][j], activate2(v[j], a.act));
-      }
-    }
-  };
-  uint32_t gate_row = 0, gate_end = a.rows;  // rows below gate_end share gate_row
-  if (!ROW_GATE && a.gate != nullptr && first < last) {
-    gate_row = first / a.period;
-    gate_end = (gate_row + 1) * a.period;
-  }
-  load_factor(gate_row);
-  const Float2x residual_scale2 = both(a.residual_scale);
-  int parity = 0;
-  for (uint32_t row = first; row < last; ++row, parity ^= 1) {
-    if (!ROW_GATE && row >= gate_end) {
-      ++gate_row;
-      gate_end += a.period;
-      load_factor(gate_row);
-    }
-    const bool landed = ring.wait();
-    const RowView xv = ring.view(a.x, a.ldx, row, landed), rv = ring.view(a.residual, a.ldr, row, landed);
-    const RowView gv = ROW_GATE ? ring.view(a.gate, a.ldgate, row, landed) : rv;
-    float r1 = 1.f;
-    if (a.post != nullptr) {
-      Float2x squares = both(0.f);
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        if (!ok[i]) continue;
-        Float2x x[P];
-        PW::load(xv, lane_in_row + i * TPR, cols, x);
-#pragma unroll
-        for (int j = 0; j < P; ++j) squares = fma_f2(x[j], x[j], squares);
-      }
-      r1 = inv_rms(row_sum<TPR, THREADS>(pair_total(squares), sums_store[group][parity][0]), a.inv_cols, a.eps);
-    }
-    const Float2x r12 = both(r1);
-    Float2x s[ITEMS][P], squares = both(0.f);
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      if (!ok[i]) continue;
-      const int w = lane_in_row + i * TPR;
-      Float2x x[P], r[P], g[P];
-      PW::load(xv, w, cols, x);
-      PW::load(rv, w, cols, r);
-      if constexpr (ROW_GATE) PW::load(gv, w, cols, g);
-#pragma unroll
-      for (int j = 0; j < P; ++j) {
-        Float2x f = factor[i][j];
-        if constexpr (ROW_GATE) f = mul_f2(f, activate2(g[j], a.act));
-        s[i][j] = fma_f2(mul_f2(r12, f), x[j], mul_f2(residual_scale2, r[j]));
-        squares = fma_f2(s[i][j], s[i][j], squares);
-      }
-      PW::store(a.s + row * a.lds, w, cols, s[i]);
-    }
-    const float r2 = inv_rms(row_sum<TPR, THREADS>(pair_total(squares), sums_store[group][parity][1]), a.inv_cols, a.eps);
-    if constexpr (TPR == 32) __syncwarp();
-    ring.release(row - first + 1);
-    if (a.stats != nullptr && lane_in_row == 0) a.stats[row] = make_float2(r1, r2);
-    const Float2x r22 = both(r2);
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      if (!ok[i]) continue;
-#pragma unroll
-      for (int j = 0; j < P; ++j) s[i][j] = mul_f2(mul_f2(s[i][j], r22), weight[i][j]);
-      PW::store(a.y + row * a.ldy, lane_in_row + i * TPR, cols, s[i]);
-    }
-  }
-  ring.finish();
-}
-
-template <typename T, bool VEC, int TPR, bool ROW_GATE>
-int launch_walk(const ForwardArgs<T>& a, const WalkPlan& p, cudaStream_t st) {
-  constexpr auto kernel = gated_walk_kernel<T, VEC, TPR, ROW_GATE>;
-  if (int rc = allow_smem<kernel>("gated_walk_kernel")) return rc;
-  launch(kernel, static_cast<unsigned>(p.ctas), TPR < 256 ? 256 : TPR, p.smem, st, a, p.walkers, p.slots, p.slot_bytes);
-  return after_launch("gated_walk_kernel");
-}
-
 template <typename T, bool VEC, int TPR, int ITEMS>
 int launch_forward(const ForwardArgs<T>& a, cudaStream_t st) {
   constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
@@ -282,27 +150,9 @@ int launch_forward(const ForwardArgs<T>& a, cudaStream_t st) {
   return after_launch("gated_add_rms_kernel");
 }
 
-template <typename T, bool VEC>
-int run_walk(const ForwardArgs<T>& a, const WalkPlan& p, bool row_gate, cudaStream_t st) {
-#define B200_WALK(TPR) return row_gate ? launch_walk<T, VEC, TPR, true>(a, p, st) : launch_walk<T, VEC, TPR, false>(a, p, st)
-  switch (p.tpr) {
-    case 32: B200_WALK(32);
-    case 128: B200_WALK(128);
-    case 256: B200_WALK(256);
-    default: B200_WALK(512);
-  }
-#undef B200_WALK
-}
-
 template <typename T>
-int run_forward(ForwardArgs<T> a, int64_t cols, bool vec, bool row_gate, cudaStream_t st) {
+int run_forward(ForwardArgs<T> a, int64_t cols, bool vec, cudaStream_t st) {
   constexpr int V = Num<T>::kVec;
-  if (cols <= kWalkColumns) {
-    const WalkPlan p = plan_walk(a.rows, cols, sizeof(T), row_gate ? 3 : 2);
-    if (p.slots > 0 && a.rows >= kWalkRows * static_cast<uint32_t>(p.walkers)) {
-      return vec ? run_walk<T, true>(a, p, row_gate, st) : run_walk<T, false>(a, p, row_gate, st);
-    }
-  }
   if (vec && cols <= 4096 * V) {
     a.words = static_cast<int>(cols / V);
     if (a.words <= 32) return launch_forward<T, true, 32, 1>(a, st);
@@ -310,6 +160,7 @@ int run_forward(ForwardArgs<T> a, int64_t cols, bool vec, bool row_gate, cudaStr
     if (a.words <= 128) return launch_forward<T, true, 32, 4>(a, st);
     if (a.words <= 256) return launch_forward<T, true, 128, 2>(a, st);
     if (a.words <= 512) return launch_forward<T, true, 256, 2>(a, st);
+    if (a.words <= 768) return launch_forward<T, true, 256, 3>(a, st);
     if (a.words <= 1024) return launch_forward<T, true, 256, 4>(a, st);
     if (a.words <= 2048) return launch_forward<T, true, 512, 4>(a, st);
     return launch_forward<T, true, 1024, 4>(a, st);
@@ -327,8 +178,6 @@ int run_forward(ForwardArgs<T> a, int64_t cols, bool vec, bool row_gate, cudaStr
 }
 
 }  // namespace
-
-unsigned int gated_norm_wait_timeouts() { return read_wait_timeouts(); }
 
 }  // namespace b200
 
@@ -365,8 +214,8 @@ extern "C" int b200_gated_add_rms_norm(const void* x, const void* residual, cons
     a.ldx = ldx, a.ldr = ldr, a.ldgate = ldgate, a.ldy = ldy, a.lds = lds;
     a.inv_cols = 1.f / static_cast<float>(cols), a.eps = static_cast<float>(eps), a.offset = static_cast<float>(offset);
     a.scale = static_cast<float>(scale), a.residual_scale = static_cast<float>(residual_scale), a.act = activation;
-    a.words = 0, a.columns = static_cast<int>(cols);
-    return run_forward<T>(a, cols, vec, gate != nullptr && gate_rows == rows && rows > 1, static_cast<cudaStream_t>(stream));
+    a.words = 0;
+    return run_forward<T>(a, cols, vec, static_cast<cudaStream_t>(stream));
   });
   return B200_OK;
 }

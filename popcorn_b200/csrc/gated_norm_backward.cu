@@ -123,7 +123,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       if (!ROW_GATE && a.gate != nullptr) {
         PW::load_shared_by_rows(a.gate + static_cast<int64_t>(gate_row) * a.ldgate, w, cols, v);
 #pragma unroll
-        for (int j = 0; j < P; ++j) factor[i][j] = mul_f2(factor[i][j], activate2(v[j], a.act));
+        for (int j = 0; j < P; ++j) factor[i][j] = mul_f2(factor[i][j], activate2<T>(v[j], a.act));
       }
     }
   };
@@ -186,7 +186,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       for (int j = 0; j < P; ++j) {
         Float2x f = factor[i][j];
         if constexpr (ROW_GATE) {
-          value[i][j] = activate2(value[i][j], a.act);
+          value[i][j] = activate2<T>(value[i][j], a.act);
           f = mul_f2(f, value[i][j]);
         }
         const Float2x u = mul_f2(f, x[j]);
@@ -305,7 +305,7 @@ gated_backward_wide_kernel(const BackwardArgs<T> a, int64_t cols, bool row_gate)
     const float c1 = a.post == nullptr ? 0.f : r1 * r1 * r1 * (inner * a.inv_cols);
     for (int64_t c = threadIdx.x; c < cols; c += kBackwardThreads) {
       const float p = a.post == nullptr ? 1.f : Num<T>::up(a.post[c]) + a.offset;
-      const float value = gr == nullptr ? 1.f : activate(Num<T>::up(gr[c]), a.act);
+      const float value = gr == nullptr ? 1.f : activate<T>(Num<T>::up(gr[c]), a.act);
       const float branch = a.scale * value, f = branch * p, x = Num<T>::up(xr[c]), gy = Num<T>::up(gyr[c]);
       const float s = stream_value<T>(x, Num<T>::up(rr[c]), f, r1, a.residual_scale);
       const float ds = fmaf(-c2, s, fmaf(r2, gy * (Num<T>::up(a.weight[c]) + a.offset), gsr == nullptr ? 0.f : Num<T>::up(gsr[c])));
@@ -359,7 +359,7 @@ gated_columns_kernel(const ColumnArgs<T> a) {
         float k = 0.f;
         for (; w < a.walkers && range_start(a.rows, a.walkers, w) < hi; ++w)
           if (range_start(a.rows, a.walkers, w + 1) > range_start(a.rows, a.walkers, w)) k += a.branch_lines[static_cast<int64_t>(w + g) * a.cols + c];
-        const float value = activate(Num<T>::up(a.gate[g * a.ldgate + c]), a.act);
+        const float value = activate<T>(Num<T>::up(a.gate[g * a.ldgate + c]), a.act);
         a.dgate[g * a.cols + c] = Num<T>::down(a.scale * p * activation_slope(value, a.act) * k);
         sum_p += a.scale * value * k;
       }
@@ -377,7 +377,7 @@ gated_columns_kernel(const ColumnArgs<T> a) {
     }
     a.dweight[c] = Num<T>::down(sum_w);
     if (a.gate_rows == 1) {
-      const float value = activate(Num<T>::up(a.gate[c]), a.act), p = a.post == nullptr ? 1.f : Num<T>::up(a.post[c]) + a.offset;
+      const float value = activate<T>(Num<T>::up(a.gate[c]), a.act), p = a.post == nullptr ? 1.f : Num<T>::up(a.post[c]) + a.offset;
       a.dgate[c] = Num<T>::down(a.scale * p * activation_slope(value, a.act) * sum_p);
       sum_p *= a.scale * value;
     }
@@ -418,6 +418,7 @@ int run_walk_back(const BackwardArgs<T>& a, const WalkPlan& p, bool row_gate, cu
 #define B200_WALK(TPR) return row_gate ? launch_backward<T, VEC, TPR, true>(a, p, st) : launch_backward<T, VEC, TPR, false>(a, p, st)
   switch (p.tpr) {
     case 32: B200_WALK(32);
+    case 64: B200_WALK(64);
     case 128: B200_WALK(128);
     case 256: B200_WALK(256);
     default: B200_WALK(512);

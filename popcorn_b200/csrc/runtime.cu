@@ -100,8 +100,7 @@ uint64_t b200_launch_count(void) { return b200::g_launches.load(std::memory_orde
 
 uint64_t b200_wait_timeouts(void) {
   return static_cast<uint64_t>(b200::rope_wait_timeouts()) + static_cast<uint64_t>(b200::norm_wait_timeouts()) +
-         static_cast<uint64_t>(b200::gemm_wait_timeouts()) + static_cast<uint64_t>(b200::gated_norm_wait_timeouts()) +
-         static_cast<uint64_t>(b200::gated_backward_wait_timeouts());
+         static_cast<uint64_t>(b200::gemm_wait_timeouts()) + static_cast<uint64_t>(b200::gated_backward_wait_timeouts());
 }
 
 }  // extern "C"
