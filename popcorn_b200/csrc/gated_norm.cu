@@ -10,8 +10,6 @@
 //
 // Bound: HBM.  Forward: x, residual (and a gate per row) read once, y and s written once.  Backward: x, residual, the
 // two incoming gradients read once, two gradients written once (s is not saved: reading residual costs the same).
-// Many rows: persistent walkers (a warp up to a CTA of 512 threads, 16 columns a thread) whose rows arrive through a ring
-// of bulk asynchronous copies in shared memory, so that the loads of the next rows are in flight while a row is reduced.
 #include "gated_norm.cuh"
 
 namespace b200 {
@@ -65,7 +63,7 @@ gated_add_rms_kernel(const ForwardArgs<T> a) {
 #pragma unroll
       for (int j = 0; j < N; ++j) sum = __fmaf_rn(f[j], f[j], sum);
     }
-    r1 = inv_rms(row_sum<TPR, THREADS>(sum, slots[0]), a.inv_cols, a.eps);
+    r1 = inv_rms(row_sum<TPR>(sum, slots[0]), a.inv_cols, a.eps);
   }
   const T* gr = a.gate == nullptr ? nullptr : a.gate + (live ? row / a.period : 0) * a.ldgate;
   float s[ITEMS][N];
@@ -95,7 +93,7 @@ gated_add_rms_kernel(const ForwardArgs<T> a) {
     }
     if (ok[i]) W::store(a.s + row * a.lds + c, s[i]);
   }
-  const float r2 = inv_rms(row_sum<TPR, THREADS>(sum, slots[1]), a.inv_cols, a.eps);
+  const float r2 = inv_rms(row_sum<TPR>(sum, slots[1]), a.inv_cols, a.eps);
   if (a.stats != nullptr && live && lane_in_row == 0) a.stats[row] = make_float2(r1, r2);
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
@@ -125,7 +123,7 @@ gated_add_rms_wide_kernel(const ForwardArgs<T> a, int64_t cols) {
       const float f = Num<T>::up(xr[c]);
       sum = __fmaf_rn(f, f, sum);
     }
-    r1 = inv_rms(row_sum<512, 512>(sum, slots[0]), a.inv_cols, a.eps);
+    r1 = inv_rms(row_sum<512>(sum, slots[0]), a.inv_cols, a.eps);
   }
   float sum = 0.f;
   for (int64_t c = threadIdx.x; c < cols; c += 512) {
@@ -133,7 +131,7 @@ gated_add_rms_wide_kernel(const ForwardArgs<T> a, int64_t cols) {
     const float s = stream_value<T>(Num<T>::up(xr[c]), Num<T>::up(rr[c]), f, r1, a.residual_scale);
     sum = __fmaf_rn(s, s, sum);
   }
-  const float r2 = inv_rms(row_sum<512, 512>(sum, slots[1]), a.inv_cols, a.eps);
+  const float r2 = inv_rms(row_sum<512>(sum, slots[1]), a.inv_cols, a.eps);
   if (a.stats != nullptr && threadIdx.x == 0) a.stats[row] = make_float2(r1, r2);
   for (int64_t c = threadIdx.x; c < cols; c += 512) {
     const float f = branch_factor(a.post, gr, c, a.offset, a.scale, a.act);

@@ -38,7 +38,7 @@ struct Word<T, false> {
 };
 
 // 16-bit types: the approximate exponential and reciprocal of activations.cuh, off by some 1e-6 of the value where T rounds
-// by 2^-11 at best; the gate of every row of [16376, 5120] fp16 costs 166 us with tanhf, 118 with this.  fp32: CUDA's own.
+// by 2^-11 at best; the gate of every row of [16376, 5120] fp16 costs 166 us with tanhf, 152 with this.  fp32: CUDA's own.
 template <typename T>
 __device__ __forceinline__ float activate(float g, int act) {
   if (act == kIdentity) return g;
@@ -61,23 +61,17 @@ __device__ __forceinline__ float activation_slope(float value, int act) {
 // 1 / sqrt(sum of squares / cols + eps), within two units in the last place (nothing is rounded to T in between)
 __device__ __forceinline__ float inv_rms(float sumsq, float inv_cols, float eps) { return rsqrtf(fmaf(sumsq, inv_cols, eps)); }
 
-// N sums over the TPR threads of a row, TPR a power of two.  Up to a warp: shuffles.  Wider: one barrier of those threads
-// (the CTA's, or a named one where several rows share the CTA); `slot` is shared memory of the row that no thread still
-// reads from an earlier call.
-template <int TPR, int THREADS>
-__device__ __forceinline__ void row_barrier() {
-  if constexpr (TPR <= 32) __syncwarp();
-  else if constexpr (TPR == THREADS) __syncthreads();
-  else asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / TPR), "r"(TPR) : "memory");
-}
-template <int TPR, int THREADS>
+// N sums over the TPR threads of a row, TPR a power of two.  Up to a warp: shuffles.  Wider: one barrier
+// (rows wider than a warp have the CTA to themselves); `slot` is shared memory that no thread still reads from an earlier
+// call.
+template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* slot) {
   v = warp_sum(v);
   if constexpr (TPR > 32) {
     constexpr int WARPS = TPR / 32;
     const int lane = threadIdx.x & 31;
-    if (lane == 0) slot[(threadIdx.x % TPR) >> 5] = v;
-    row_barrier<TPR, THREADS>();
+    if (lane == 0) slot[threadIdx.x >> 5] = v;
+    __syncthreads();
     v = slot[lane & (WARPS - 1)];
 #pragma unroll
     for (int o = WARPS / 2; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -86,7 +80,7 @@ __device__ __forceinline__ float row_sum(float v, float* slot) {
 }
 // Four at once: two steps leave each lane with a quarter of the lanes' sum of one value (value 2 (lane / 8 % 2) + lane / 16),
 // so six exchanges do for four sums, where one after the other takes twenty.
-template <int TPR, int THREADS>
+template <int TPR>
 __device__ __forceinline__ void row_sums(float (&v)[4], float (*slot)[16]) {
   const int lane = threadIdx.x & 31;
   const bool high = lane & 16, odd = lane & 8;
@@ -97,8 +91,8 @@ __device__ __forceinline__ void row_sums(float (&v)[4], float (*slot)[16]) {
   for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if constexpr (TPR > 32) {
     constexpr int WARPS = TPR / 32;
-    if ((lane & 7) == 0) slot[(odd ? 2 : 0) + (high ? 1 : 0)][(threadIdx.x % TPR) >> 5] = sum;
-    row_barrier<TPR, THREADS>();
+    if ((lane & 7) == 0) slot[(odd ? 2 : 0) + (high ? 1 : 0)][threadIdx.x >> 5] = sum;
+    __syncthreads();
     const float* mine = slot[(odd ? 2 : 0) + (high ? 1 : 0)];
     sum = mine[lane & (WARPS < 8 ? WARPS - 1 : 7)];
     if constexpr (WARPS == 16) sum += mine[8 + (lane & 7)];
@@ -140,10 +134,10 @@ struct RowView {
   const void* row;
 };
 
-template <typename T, bool VEC, int TPR, int THREADS>
+template <typename T, bool VEC, int TPR>
 struct Ring {
   uint32_t full, memory;  // shared-memory addresses
-  volatile int* broken;
+  uint32_t broken;  // shared-memory address of the walker's flag
   int count, slots, rows_ahead;
   uint32_t row_bytes, slot_bytes;
   // the issuing threads (the first `count` of the walker, one array each): their array and the next row of it
@@ -158,19 +152,24 @@ struct Ring {
   // memory: slots * slot_bytes of this walker; all threads of the CTA call this.  array(a, base, ld) names the rows of array a.
   template <typename Arrays>
   __device__ __forceinline__ void start(uint64_t* barriers, unsigned char* mem, int* flag, int n, uint32_t bytes, uint32_t padded, uint32_t first, uint32_t last, int arrays, Arrays&& array) {
-    full = smem_addr(barriers), memory = smem_addr(mem), broken = flag;
+    full = smem_addr(barriers), memory = smem_addr(mem), broken = smem_addr(flag);
     count = arrays, slots = n, row_bytes = bytes, slot_bytes = padded, put_row = first_row = first, last_row = last;
     rows_ahead = (slots + count - 1) / count;  // a barrier is used again only after the row before was given free
-    put_copy = put = threadIdx.x % TPR;
+    put_copy = put = threadIdx.x;
     put_bar = take = take_bar = 0, phase = 0;
-    array(static_cast<int>(put_copy), base, ld);
-    if (threadIdx.x % TPR == 0) {
-      *broken = 0;
+    array(static_cast<int>(threadIdx.x), base, ld);
+    if (threadIdx.x == 0) {
+      *flag = 0;
       for (int k = 0; k < rows_ahead; ++k) mbar_init(barriers + k, count);
       mbar_init_fence();
     }
     __syncthreads();
-    if (threadIdx.x % TPR < count) issue(slots);
+    if (threadIdx.x < count) issue(slots);
+  }
+  __device__ __forceinline__ bool is_broken() const {
+    uint32_t v;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(broken) : "memory");
+    return v != 0;
   }
   // bytes of a row that the ring holds, from the row's start
   __device__ __forceinline__ void span(const T* row, uint32_t& lo, uint32_t& hi) const {
@@ -202,7 +201,7 @@ struct Ring {
   }
   // the walker is past a barrier behind its last read of the first `rows` rows
   __device__ __forceinline__ void release(uint32_t rows) {
-    if (threadIdx.x % TPR < count && *broken == 0) issue(static_cast<int64_t>(rows) * count + slots);
+    if (threadIdx.x < count && !is_broken()) issue(static_cast<int64_t>(rows) * count + slots);
   }
   static __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
     for (uint32_t i = 0; i < kSpinLimit; ++i) {
@@ -221,9 +220,9 @@ struct Ring {
   }
   // the next row in turn: has it landed?
   __device__ __forceinline__ bool wait() {
-    bool landed = *broken == 0;
+    bool landed = !is_broken();
     if (landed && !wait_for(full + take_bar * 8, phase)) {
-      *broken = 1;
+      asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(broken), "r"(1) : "memory");
       landed = false;
     }
     if (++take_bar == rows_ahead) {
@@ -240,7 +239,7 @@ struct Ring {
     if constexpr (VEC) {
       if (!landed) {
         const unsigned char* bytes = reinterpret_cast<const unsigned char*>(from + row * stride);
-        for (uint32_t at = (threadIdx.x % TPR) * 16u; at < row_bytes; at += TPR * 16u) st_shared(v.memory + at, ld_stream(bytes + at));
+        for (uint32_t at = (threadIdx.x) * 16u; at < row_bytes; at += TPR * 16u) st_shared(v.memory + at, ld_stream(bytes + at));
       }
     } else {
       v.row = from + row * stride;
@@ -252,7 +251,7 @@ struct Ring {
   }
   // before the walker's memory is left
   __device__ __forceinline__ void finish() {
-    if (threadIdx.x % TPR == 0 && *broken != 0) {
+    if (threadIdx.x == 0 && is_broken()) {
       const uint32_t rows = put_row - first_row;
       for (uint32_t r = rows > static_cast<uint32_t>(rows_ahead) ? rows - rows_ahead : 0; r < rows; ++r) (void)wait_for(full + r % rows_ahead * 8, r / rows_ahead & 1u);
     }
@@ -328,7 +327,7 @@ __device__ __forceinline__ Float2x activate2(Float2x g, int act) {
 constexpr int kColumns = 16;  // columns per thread of a walker
 constexpr int kMaxWalk = 512;
 constexpr int kWalkColumns = kMaxWalk * kColumns;
-constexpr int kMaxRingBytes = 208 * 1024;
+constexpr int kRingBytes = 196 * 1024;  // of an SM; the rest of its 228 KB is what 16 CTAs need besides
 
 // s of one element, for the kernels that go over a row more than once
 template <typename T>
@@ -344,25 +343,20 @@ __device__ __forceinline__ float branch_factor(const T* post, const T* gate_row,
   return f;
 }
 
-// The threads of a walker for a row of `cols`, its rows' slots in shared memory, and how many walkers share `rows`.
+// The threads of a walker for a row of `cols`, its rows' slots in shared memory, and how many walkers share `rows`: as many
+// as give an SM 512 threads of 128 registers.
 struct WalkPlan {
-  int tpr, walkers, ctas, slots;
+  int tpr, walkers, slots;
   uint32_t slot_bytes;
-  size_t smem;
 };
-WalkPlan plan_walk(int64_t rows, int64_t cols, size_t element, int arrays) {
+WalkPlan plan_walk(int64_t rows, int64_t cols, size_t element) {
   WalkPlan p;
   p.tpr = 32;
   while (p.tpr * kColumns < cols) p.tpr *= 2;
-  const int groups = p.tpr < 256 ? 256 / p.tpr : 1, per_sm = p.tpr < 512 ? 2 : 1;
-  const int64_t most = static_cast<int64_t>(sm_count()) * per_sm * groups;
-  p.walkers = static_cast<int>(std::max<int64_t>(1, std::min(rows, most)));
-  p.ctas = static_cast<int>(ceil_div(p.walkers, groups));
+  const int per_sm = kMaxWalk / p.tpr;
+  p.walkers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, static_cast<int64_t>(sm_count()) * per_sm)));
   p.slot_bytes = static_cast<uint32_t>(std::max<int64_t>(1, ceil_div(cols * static_cast<int64_t>(element), 16)) * 16);
-  const size_t budget = (per_sm == 2 ? 100 : 208) * 1024 / groups;
-  p.slots = static_cast<int>(std::min<size_t>(kMaxSlots, budget / p.slot_bytes));
-  p.smem = static_cast<size_t>(p.slots) * p.slot_bytes * groups;
-  if (p.slots < arrays) p.slots = 0;
+  p.slots = static_cast<int>(std::min<size_t>(kMaxSlots, kRingBytes / per_sm / p.slot_bytes));  // at least 6: a row's arrays fit
   return p;
 }
 
@@ -374,7 +368,7 @@ int allow_smem(const char* name) {
   if (cudaGetDevice(&device) != cudaSuccess) return fail(B200_ERR_DEVICE, "%s: no current device", name);
   const uint64_t bit = device < 64 ? 1ull << device : 0;
   if (done.load(std::memory_order_acquire) & bit) return B200_OK;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRingBytes) != cudaSuccess)
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes) != cudaSuccess)
     return fail(B200_ERR_LAUNCH, "%s: %s", name, cudaGetErrorString(cudaGetLastError()));
   done.fetch_or(bit, std::memory_order_release);
   return B200_OK;

@@ -10,8 +10,9 @@
 //   grad_gate = scale act'(gate) (post_weight + offset) k,  grad_post_weight = sum over gate rows of a k
 //   A gate of its own for each row has its gradient written with the row, and a k is summed instead of k.
 //
-// Each walker goes over a contiguous range of rows with the sums of its columns in registers; at the end every CTA writes
-// a line of its walkers' sums to scratch.  With several gate rows a walker also writes a line of k whenever the gate row
+// A walker (a CTA of 32 to 512 threads, 16 columns a thread) goes over a contiguous range of rows, which arrive through a
+// ring of bulk copies in shared memory, with the sums of its columns in registers, and writes a line of them to scratch at
+// its end.  With several gate rows a walker also writes a line of k whenever the gate row
 // changes, at index walker + gate row, which no other pair (walker, gate row) has.  gated_columns_kernel adds the lines up
 // in a fixed order: the result does not depend on timing.
 #include "gated_norm.cuh"
@@ -29,64 +30,27 @@ struct BackwardArgs {
   float *weight_lines, *branch_lines;
   uint32_t rows, period;
   int columns, walkers;
-  bool by_group;  // several gate rows, each shared by several rows
   int64_t ldgy, ldgs, ldx, ldr, ldgate, ldo;
   float inv_cols, offset, scale, residual_scale;
   int act;
 };
 
-// The sums of a walker's columns end in lines of scratch.  The groups of a CTA are added up in order first, so that a
-// line is one CTA's.
-template <int TPR, int THREADS, int ITEMS, int P, int N>
-__device__ __forceinline__ void fold_line(const Float2x (&sums)[ITEMS][P], const bool (&ok)[ITEMS], float* fold, float* line, int64_t cols) {
-  constexpr int GROUPS = THREADS / TPR;
-  const int group = threadIdx.x / TPR, lane_in_row = threadIdx.x % TPR;
-  for (int g = 0; g < GROUPS; ++g) {
-    if (group == g) {
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        if (!ok[i]) continue;
-        const int c = (lane_in_row + i * TPR) * N;
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-          float v[2];
-          unpack_f2(sums[i][j], v[0], v[1]);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (c + 2 * j + k >= cols) break;
-            float* to = GROUPS == 1 ? line + c + 2 * j + k : fold + c + 2 * j + k;
-            *to = g == 0 ? v[k] : __fadd_rn(*to, v[k]);
-          }
-        }
-      }
-    }
-    if (GROUPS > 1) __syncthreads();
-  }
-  if (GROUPS > 1) {
-    for (int64_t c = threadIdx.x; c < cols; c += THREADS) line[c] = fold[c];
-    __syncthreads();
-  }
-}
-
 template <typename T, bool VEC, int TPR, bool ROW_GATE>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 2 : 1)
+__global__ void __launch_bounds__(TPR, kMaxWalk / TPR)
 gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
   using PW = Pairs<T, VEC>;
   constexpr int N = PW::N, P = PW::P, ITEMS = kColumns / N;
-  constexpr int THREADS = TPR < 256 ? 256 : TPR, GROUPS = THREADS / TPR;
   const int cols = a.columns, words = (cols + N - 1) / N;
   extern __shared__ __align__(128) unsigned char memory[];
-  __shared__ uint64_t barriers[GROUPS][kMaxSlots];
-  __shared__ int flags[GROUPS];
-  __shared__ float sums_store[GROUPS][2][4][16];
-  __shared__ float fold[GROUPS > 1 ? TPR * kColumns : 1];
+  __shared__ uint64_t barriers[kMaxSlots];
+  __shared__ int flag;
+  __shared__ float sums_store[2][4][16];
   pdl_prologue();
-  const int group = threadIdx.x / TPR, lane_in_row = threadIdx.x % TPR;
-  const int walker = blockIdx.x * GROUPS + group;
-  const uint32_t first = walker < a.walkers ? range_start(a.rows, a.walkers, walker) : 0, last = walker < a.walkers ? range_start(a.rows, a.walkers, walker + 1) : 0;
-  Ring<T, VEC, TPR, THREADS> ring;
+  const int lane_in_row = threadIdx.x, walker = blockIdx.x;
+  const uint32_t first = range_start(a.rows, a.walkers, walker), last = range_start(a.rows, a.walkers, walker + 1);
+  Ring<T, VEC, TPR> ring;
   const bool has_gs = a.gs != nullptr;
-  ring.start(barriers[group], memory + static_cast<size_t>(group) * slots * slot_bytes, &flags[group], slots, static_cast<uint32_t>(cols) * sizeof(T), slot_bytes, first, last, 3 + (ROW_GATE ? 1 : 0) + (has_gs ? 1 : 0),
+  ring.start(barriers, memory, &flag, slots, static_cast<uint32_t>(cols) * sizeof(T), slot_bytes, first, last, 3 + (ROW_GATE ? 1 : 0) + (has_gs ? 1 : 0),
              [&](int array, const T*& base, int64_t& ld) {
                base = array == 0 ? a.x : array == 1 ? a.residual : array == 2 ? a.gy : ROW_GATE && array == 3 ? a.gate : a.gs;
                ld = array == 0 ? a.ldx : array == 1 ? a.ldr : array == 2 ? a.ldgy : ROW_GATE && array == 3 ? a.ldgate : a.ldgs;
@@ -127,7 +91,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       }
     }
   };
-  auto write_line = [&](float* line) {
+  auto write_line = [&](float* line, const Float2x (&sums)[ITEMS][P]) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       if (!ok[i]) continue;
@@ -135,7 +99,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         float lo, hi;
-        unpack_f2(sum_k[i][j], lo, hi);
+        unpack_f2(sums[i][j], lo, hi);
         line[c + 2 * j] = lo;
         if (c + 2 * j + 1 < cols) line[c + 2 * j + 1] = hi;
       }
@@ -153,7 +117,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
   int parity = 0;
   for (uint32_t row = first; row < last; ++row, parity ^= 1) {
     if (!ROW_GATE && row >= gate_end) {
-      write_line(a.branch_lines + static_cast<int64_t>(walker + gate_row) * cols);
+      write_line(a.branch_lines + static_cast<int64_t>(walker + gate_row) * cols, sum_k);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
@@ -189,8 +153,8 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
           value[i][j] = activate2<T>(value[i][j], a.act);
           f = mul_f2(f, value[i][j]);
         }
-        const Float2x u = mul_f2(f, x[j]);
-        const Float2x s = fma_f2(r12, u, mul_f2(residual_scale2, res[j]));
+        const Float2x u = mul_f2(f, mul_f2(r12, x[j]));
+        const Float2x s = fma_f2(residual_scale2, res[j], u);
         const Float2x gw = mul_f2(gy[j], weight[i][j]);
         acc[0] = fma_f2(gw, s, acc[0]);
         acc[1] = fma_f2(u, gs[j], acc[1]);
@@ -201,13 +165,13 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
     float sums[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) sums[n] = pair_total(acc[n]);
-    row_sums<TPR, THREADS>(sums, sums_store[group][parity]);
+    row_sums<TPR>(sums, sums_store[parity]);
     // every thread of the walker is past the row before: its slots can be filled again
     if (TPR > 32 && !tight) ring.release(row - first);
     const float c2 = r2 * r2 * r2 * (sums[0] * a.inv_cols);
+    // sums 1 to 3 hold r1 f x, and grad_x takes r1 x: c1 = r1^2 (r1 <f ds, x>) / cols, c1 x = (c1 / r1) r1 x
     const float inner = sums[1] + r2 * sums[2] - c2 * sums[3];
-    const float c1 = a.post == nullptr ? 0.f : r1 * r1 * r1 * (inner * a.inv_cols);
-    const Float2x minus_c2 = both(-c2), minus_c1 = both(-c1);
+    const Float2x minus_c2 = both(-c2), minus_c1 = both(a.post == nullptr ? 0.f : -r1 * (inner * a.inv_cols));
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       if (!ok[i]) continue;
@@ -224,20 +188,20 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       for (int j = 0; j < P; ++j) {
         Float2x f = factor[i][j];
         if constexpr (ROW_GATE) f = mul_f2(f, value[i][j]);
-        const Float2x s = fma_f2(r12, mul_f2(f, x[j]), mul_f2(residual_scale2, res[j]));
-        const Float2x ds = fma_f2(minus_c2, s, fma_f2(r22, mul_f2(gy[j], weight[i][j]), gs[j]));
-        const Float2x dsx = mul_f2(ds, x[j]);
-        sum_w[i][j] = fma_f2(mul_f2(gy[j], s), r22, sum_w[i][j]);
+        const Float2x xr = mul_f2(r12, x[j]), gr = mul_f2(r22, gy[j]);
+        const Float2x s = fma_f2(residual_scale2, res[j], mul_f2(f, xr));
+        const Float2x ds = fma_f2(minus_c2, s, fma_f2(gr, weight[i][j], gs[j]));
+        sum_w[i][j] = fma_f2(gr, s, sum_w[i][j]);
         if constexpr (ROW_GATE) {
-          const Float2x k = mul_f2(dsx, r12);
+          const Float2x k = mul_f2(ds, xr);
           sum_k[i][j] = fma_f2(mul_f2(scale2, value[i][j]), k, sum_k[i][j]);
           float lo, hi;
           unpack_f2(value[i][j], lo, hi);
           g[j] = mul_f2(mul_f2(factor[i][j], pack_f2(activation_slope(lo, a.act), activation_slope(hi, a.act))), k);
         } else {
-          sum_k[i][j] = fma_f2(dsx, r12, sum_k[i][j]);
+          sum_k[i][j] = fma_f2(ds, xr, sum_k[i][j]);
         }
-        x[j] = fma_f2(mul_f2(r12, f), ds, mul_f2(minus_c1, x[j]));
+        x[j] = fma_f2(f, mul_f2(r12, ds), mul_f2(minus_c1, xr));
         res[j] = mul_f2(residual_scale2, ds);
       }
       PW::store(a.dx + at, w, cols, x);
@@ -245,17 +209,13 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       if constexpr (ROW_GATE) PW::store(a.dgate + at, w, cols, g);
     }
     if (TPR == 32 || tight) {
-      row_barrier<TPR, THREADS>();
+      __syncthreads();
       ring.release(row - first + 1);
     }
   }
   ring.finish();
-  if (a.by_group) {
-    if (first < last) write_line(a.branch_lines + static_cast<int64_t>(walker + gate_row) * cols);
-  } else if (a.branch_lines != nullptr) {
-    fold_line<TPR, THREADS, ITEMS, P, N>(sum_k, ok, fold, a.branch_lines + blockIdx.x * cols, cols);
-  }
-  fold_line<TPR, THREADS, ITEMS, P, N>(sum_w, ok, fold, a.weight_lines + blockIdx.x * cols, cols);
+  write_line(a.weight_lines + static_cast<int64_t>(walker) * cols, sum_w);
+  if (a.branch_lines != nullptr) write_line(a.branch_lines + static_cast<int64_t>(walker + gate_row) * cols, sum_k);
 }
 
 // Any width: one CTA per walker, the row read twice, the sums of a walker's columns kept in its lines in scratch.
@@ -276,7 +236,7 @@ gated_backward_wide_kernel(const BackwardArgs<T> a, int64_t cols, bool row_gate)
     if (sum_k != nullptr)
       for (int64_t c = threadIdx.x; c < cols; c += kBackwardThreads) sum_k[c] = 0.f;
   };
-  if (!a.by_group || first < last) clear_k();
+  clear_k();
   int parity = 0;
   for (uint32_t row = first; row < last; ++row, parity ^= 1) {
     if (shared_gate && row / a.period != gate_row) {
@@ -299,7 +259,7 @@ gated_backward_wide_kernel(const BackwardArgs<T> a, int64_t cols, bool row_gate)
       sums[2] = fmaf(u, gw, sums[2]);
       sums[3] = fmaf(u, s, sums[3]);
     }
-    row_sums<kBackwardThreads, kBackwardThreads>(sums, slots[parity]);
+    row_sums<kBackwardThreads>(sums, slots[parity]);
     const float c2 = r2 * r2 * r2 * (sums[0] * a.inv_cols);
     const float inner = sums[1] + r2 * sums[2] - c2 * sums[3];
     const float c1 = a.post == nullptr ? 0.f : r1 * r1 * r1 * (inner * a.inv_cols);
@@ -330,7 +290,7 @@ struct ColumnArgs {
   T *dweight, *dpost, *dgate;
   int64_t cols, ldgate;
   uint32_t rows, period;
-  int weight_count, walkers, gate_rows;  // gate_rows: 0 unless rows share gate rows
+  int walkers, gate_rows;  // gate_rows: 0 unless rows share gate rows
   float offset, scale, line_scale;  // line_scale: what a sum over branch_lines lacks of grad_post_weight
   int act;
 };
@@ -343,12 +303,23 @@ gated_columns_kernel(const ColumnArgs<T> a) {
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float sum_w = 0.f, sum_p = 0.f;
   if (c < a.cols) {
-#pragma unroll 10
-    for (int l = warp; l < a.weight_count; l += kColumnWarps) sum_w += a.weight_lines[l * a.cols + c];
-    if (a.branch_lines != nullptr && a.gate_rows <= 1) {
-#pragma unroll 10
-      for (int l = warp; l < a.weight_count; l += kColumnWarps) sum_p += a.branch_lines[l * a.cols + c];
-    } else if (a.branch_lines != nullptr) {
+    const bool branch = a.branch_lines != nullptr && a.gate_rows <= 1;
+    constexpr int BATCH = 8;  // loads of either kind in flight
+    for (int l0 = warp; l0 < a.walkers; l0 += BATCH * kColumnWarps) {
+      float w[BATCH], p[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int l = l0 + k * kColumnWarps;
+        w[k] = l < a.walkers ? a.weight_lines[l * a.cols + c] : 0.f;
+        p[k] = branch && l < a.walkers ? a.branch_lines[l * a.cols + c] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        sum_w += w[k];
+        sum_p += p[k];
+      }
+    }
+    if (a.branch_lines != nullptr && a.gate_rows > 1) {
       const float p = a.post == nullptr ? 1.f : Num<T>::up(a.post[c]) + a.offset;
       for (int g = warp; g < a.gate_rows; g += kColumnWarps) {
         // walkers whose rows meet this gate row's: those from the one that holds its first row to the one that holds its last
@@ -396,12 +367,12 @@ BackwardPlan plan_backward(int64_t rows, int64_t cols, int64_t gate_rows, size_t
   p.walk = cols <= kWalkColumns;
   const bool by_group = gate_rows > 1 && gate_rows < rows;
   if (p.walk) {
-    p.w = plan_walk(rows, cols, element, kMaxArrays);
+    p.w = plan_walk(rows, cols, element);
   } else {
-    p.w.walkers = p.w.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, static_cast<int64_t>(sm_count()) * 2)));
+    p.w.walkers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, static_cast<int64_t>(sm_count()) * 2)));
   }
-  p.weight_lines = p.w.ctas;
-  p.branch_lines = by_group ? p.w.walkers + gate_rows : p.w.ctas;
+  p.weight_lines = p.w.walkers;
+  p.branch_lines = p.w.walkers + (by_group ? gate_rows : 0);
   return p;
 }
 
@@ -409,7 +380,7 @@ template <typename T, bool VEC, int TPR, bool ROW_GATE>
 int launch_backward(const BackwardArgs<T>& a, const WalkPlan& p, cudaStream_t st) {
   constexpr auto kernel = gated_backward_kernel<T, VEC, TPR, ROW_GATE>;
   if (int rc = allow_smem<kernel>("gated_backward_kernel")) return rc;
-  launch(kernel, static_cast<unsigned>(p.ctas), TPR < 256 ? 256 : TPR, p.smem, st, a, p.slots, p.slot_bytes);
+  launch(kernel, static_cast<unsigned>(p.walkers), TPR, static_cast<size_t>(p.slots) * p.slot_bytes, st, a, p.slots, p.slot_bytes);
   return after_launch("gated_backward_kernel");
 }
 
@@ -515,7 +486,7 @@ extern "C" int b200_gated_add_rms_norm_backward(const void* grad_y, const void* 
     a.weight_lines = static_cast<float*>(scratch);
     a.branch_lines = post_weight == nullptr && !shared_gate ? nullptr : a.weight_lines + p.weight_lines * cols;
     a.rows = static_cast<uint32_t>(rows), a.period = shared_gate ? static_cast<uint32_t>(rows / gate_rows) : 1;
-    a.columns = static_cast<int>(cols), a.walkers = p.w.walkers, a.by_group = shared_gate && gate_rows > 1;
+    a.columns = static_cast<int>(cols), a.walkers = p.w.walkers;
     a.ldgy = ldgy, a.ldgs = ldgs, a.ldx = ldx, a.ldr = ldr, a.ldgate = ldgate, a.ldo = cols;
     a.inv_cols = 1.f / static_cast<float>(cols), a.offset = static_cast<float>(offset), a.scale = static_cast<float>(scale);
     a.residual_scale = static_cast<float>(residual_scale), a.act = activation;
@@ -523,7 +494,7 @@ extern "C" int b200_gated_add_rms_norm_backward(const void* grad_y, const void* 
     c.weight_lines = a.weight_lines, c.branch_lines = a.branch_lines, c.post = a.post, c.gate = a.gate;
     c.dweight = static_cast<T*>(grad_weight), c.dpost = static_cast<T*>(grad_post_weight), c.dgate = a.dgate;
     c.cols = cols, c.ldgate = ldgate, c.rows = a.rows, c.period = a.period;
-    c.weight_count = p.w.ctas, c.walkers = p.w.walkers, c.gate_rows = shared_gate ? static_cast<int>(gate_rows) : 0;
+    c.walkers = p.w.walkers, c.gate_rows = shared_gate ? static_cast<int>(gate_rows) : 0;
     c.offset = a.offset, c.scale = a.scale, c.line_scale = gate == nullptr ? a.scale : 1.f, c.act = activation;
     return run_backward<T>(a, c, cols, p, words, row_gate, static_cast<cudaStream_t>(stream));
   });
