@@ -392,7 +392,7 @@ int b200_moe_route(const void* logits, int32_t* indices, float* weights,
  * logits: [groups * tokens, experts] (ld_logits elements per row); indices: int32 [groups * tokens, top_k], the picks of
  * b200_moe_route.  stats: fp32 [groups * tokens][2] (row maximum and sum, written for kept rows) or NULL; table: fp32
  * [groups * (experts + 1) + 1]; the backward reads both.  Limits: experts <= 1024, top_k <= min(experts, 32), groups <=
- * 65535, fewer than 2^31 picks.  scratch: b200_moe_balance_scratch_bytes() bytes, 16-byte aligned, not to be shared by
+ * 65535, at most 2^30 picks.  scratch: b200_moe_balance_scratch_bytes() bytes, 16-byte aligned, not to be shared by
  * calls that may run at the same time.  Sums are fp32 within a CTA and fp64 over the CTAs, in a fixed order.
  *
  * popcorn's momoe takes router logits and has no such loss (src/popcorn/kernels/momoe.py:34-53).
