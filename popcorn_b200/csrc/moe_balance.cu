@@ -13,6 +13,7 @@
 // pass (8 bytes a token).  A lane has eight loads in flight, of one token or of several: with two, [131072, 256] fp32 took
 // 91 us forward instead of 35.
 #include <algorithm>
+#include <type_traits>
 
 #include "activations.cuh"
 #include "common.cuh"
@@ -31,6 +32,10 @@ template <typename T>
 struct Load<T, true> {
   static constexpr int N = Num<T>::kVec;
   using Raw = uint4;
+  static __device__ __forceinline__ Raw lowest() {  // -inf throughout
+    const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    return make_uint4(w, w, w, w);
+  }
   static __device__ __forceinline__ Raw get(const T* p) { return ld_stream(p); }
   static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[N]) { Num<T>::unpack(r, f); }
   static __device__ __forceinline__ void put(T* p, const float (&f)[N]) { st_stream(p, Num<T>::pack(f)); }
@@ -39,6 +44,7 @@ template <typename T>
 struct Load<T, false> {
   static constexpr int N = 1;
   using Raw = T;
+  static __device__ __forceinline__ Raw lowest() { return Num<T>::down(-INFINITY); }
   static __device__ __forceinline__ Raw get(const T* p) { return *p; }
   static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[1]) { f[0] = Num<T>::up(r); }
   static __device__ __forceinline__ void put(T* p, const float (&f)[1]) { *p = Num<T>::down(f[0]); }
@@ -114,10 +120,15 @@ balance_sums_kernel(const T* logits, const int32_t* indices, const uint8_t* mask
       kept_next[u] = t < tokens && (mask == nullptr || mask[t] != 0);
     }
   };
+  // loads behind the last expert are never made and stay -inf; those of a token that does not count are stale and not used
+  typename L::Raw raw[U][WPL];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < WPL; ++i) raw[u][i] = L::lowest();
   look(blockIdx.x);
   for (int64_t tile = blockIdx.x; tile * TILE < tokens; tile += s.chunks) {
     const int t0 = static_cast<int>(tile) * TILE + warp * TOKENS * U;
-    typename L::Raw raw[U][WPL];
     bool keep[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -149,9 +160,7 @@ balance_sums_kernel(const T* logits, const int32_t* indices, const uint8_t* mask
       float v[WPL][N], top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < WPL; ++i) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[i][j] = -INFINITY;
-        if (keep[u] && (lane_in_token + i * LPT) * N < s.experts) L::unpack(raw[u][i], v[i]);
+        L::unpack(raw[u][i], v[i]);
 #pragma unroll
         for (int j = 0; j < N; ++j) top = fmaxf(top, v[i][j]);
       }
@@ -159,10 +168,9 @@ balance_sums_kernel(const T* logits, const int32_t* indices, const uint8_t* mask
       float total = 0.f;
 #pragma unroll
       for (int i = 0; i < WPL; ++i) {
-        const bool there = (lane_in_token + i * LPT) * N < s.experts;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          v[i][j] = there ? exp_from(v[i][j], top) : 0.f;  // a row of -inf alone is NaN, as in a softmax
+          v[i][j] = exp_from(v[i][j], top);  // a row of -inf alone is NaN, as in a softmax
           total += v[i][j];
         }
       }
@@ -259,14 +267,7 @@ balance_group_kernel(const Shape s, const Partials in, int groups, int cluster, 
     z += in.z[line0 + c];
     n += in.kept[line0 + c];
   }
-  z = warp_sum_f64(z);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  if (lane == 0) {
-    fold_z[warp] = z;
-    fold_n[warp] = n;
-  }
-  double balance = 0.0;  // of warp 0's lanes
+  double balance = 0.0;  // of each warp's first lane
   for (int e0 = rank * 32; e0 < s.experts; e0 += cluster * 32) {
     const int e = e0 + lane;
     double p = 0.0;
@@ -291,6 +292,15 @@ balance_group_kernel(const Shape s, const Partials in, int groups, int cluster, 
     __syncthreads();  // the round before has been read
     fold_p[warp][lane] = p;
     fold_c[warp][lane] = picks;
+    if (e0 == rank * 32) {  // here, and not before the first loads were asked for
+      z = warp_sum_f64(z);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      if (lane == 0) {
+        fold_z[warp] = z;
+        fold_n[warp] = n;
+      }
+    }
     __syncthreads();
     // warp w adds up what the warps have of expert w of the 32
     p = warp_sum_f64(fold_p[lane][warp]);
@@ -415,10 +425,15 @@ balance_backward_kernel(const T* logits, const uint8_t* mask, const float2* stat
       kept_next[u] = t < tokens && (mask == nullptr || mask[t] != 0);
     }
   };
+  // loads behind the last expert are never made and stay -inf; those of a token that does not count are stale and not used
+  typename L::Raw raw[U][WPL];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < WPL; ++i) raw[u][i] = L::lowest();
   look(blockIdx.x);
   for (int64_t tile = blockIdx.x; tile * TILE < tokens; tile += s.chunks) {
     const int t0 = static_cast<int>(tile) * TILE + warp * TOKENS * U;
-    typename L::Raw raw[U][WPL];
     float2 stat[U];
     bool keep[U];
 #pragma unroll
@@ -441,13 +456,10 @@ balance_backward_kernel(const T* logits, const uint8_t* mask, const float2* stat
       float inner = 0.f;
 #pragma unroll
       for (int i = 0; i < WPL; ++i) {
-        const bool there = (lane_in_token + i * LPT) * N < s.experts;
-#pragma unroll
-        for (int j = 0; j < N; ++j) p[i][j] = -INFINITY;
-        if (keep[u] && there) L::unpack(raw[u][i], p[i]);
+        L::unpack(raw[u][i], p[i]);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          p[i][j] = there ? exp_from(p[i][j], stat[u].x) * inv : 0.f;
+          p[i][j] = exp_from(p[i][j], stat[u].x) * inv;
           inner = fmaf(p[i][j], f[i][j], inner);
         }
       }
