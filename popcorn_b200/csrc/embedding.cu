@@ -82,27 +82,44 @@ embedding_kernel(const I* ids, const T* weight, T* out, int64_t tokens, int64_t 
 template <typename T, typename I>
 __global__ void __launch_bounds__(kOrderThreads)
 embedding_order_kernel(const I* ids, int tokens, int64_t vocab, int padding, int range, int32_t* token,
-                       int32_t* id, int32_t* count, T* grad_weight, int64_t cols, bool vec) {
+                       int32_t* id, int32_t* count, T* grad_weight, int64_t cols) {
+  constexpr int AHEAD = 8;
   extern __shared__ int place[];  // [warp][row of the range]: first the warp's tokens of the row, then where they go
   __shared__ int totals[kMaxRange];
   __shared__ int fold[kOrderWarps];
+  __shared__ int next_row;
   pdl_prologue();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t first_row = static_cast<int64_t>(blockIdx.x) * range;
   const int rows = static_cast<int>(min(static_cast<int64_t>(range), vocab - first_row));
+  if (threadIdx.x == 0) next_row = 0;
   for (int i = threadIdx.x; i < kOrderWarps * range; i += kOrderThreads) place[i] = 0;
   __syncthreads();
-  // every warp has a contiguous piece of the ids, so that warp order is token order
+  // the ids in one contiguous piece per warp, so that piece order is token order
   const int piece = (tokens + kOrderWarps - 1) / kOrderWarps;
-  const int begin = min(tokens, warp * piece), end = min(tokens, begin + piece);
+  auto piece_start = [&](int p) { return static_cast<int>(min(static_cast<int64_t>(tokens), static_cast<int64_t>(p) * piece)); };
+  const int begin = piece_start(warp), end = piece_start(warp + 1);
   int below = 0;
-#pragma unroll 4
-  for (int t = begin + lane; t < end; t += 32) {
-    const int row = row_of(ids[t], vocab);
-    if (row < 0 || row == padding) continue;
-    const int64_t at = row - first_row;
-    if (at < 0) ++below;
-    else if (at < rows) atomicAdd(&place[warp * range + at], 1);
+  // the rows of eight batches of a warp's tokens at a time; -1: none, also for padding
+  int row[AHEAD];
+  auto fetch = [&](int t0, int stop) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int t = t0 + k * 32 + lane;
+      row[k] = t < stop ? row_of(ids[t], vocab) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (row[k] == padding) row[k] = -1;
+  };
+  for (int t0 = begin; t0 < end; t0 += 32 * AHEAD) {
+    fetch(t0, end);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int64_t at = row[k] - first_row;
+      if (row[k] >= 0 && at < 0) ++below;
+      if (at >= 0 && at < rows) atomicAdd(&place[warp * range + at], 1);
+    }
   }
   below = __reduce_add_sync(0xffffffffu, below);
   if (lane == 0) fold[warp] = below;
@@ -142,32 +159,46 @@ embedding_order_kernel(const I* ids, int tokens, int64_t vocab, int padding, int
   }
   if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *count = start + all;
   __syncthreads();
-  for (int t0 = begin; t0 < end; t0 += 32) {
-    const int t = t0 + lane;
-    const int row = t < end ? row_of(ids[t], vocab) : -1;
-    const int64_t at = row - first_row;
-    const bool here = row >= 0 && row != padding && at >= 0 && at < rows;
-    const unsigned active = __ballot_sync(0xffffffffu, here);
-    if (here) {
-      const unsigned same = __match_any_sync(active, row);
-      const int rank = __popc(same & ((1u << lane) - 1));
-      const int to = place[warp * range + at] + rank;
-      __syncwarp(active);
-      if (rank == 0) place[warp * range + at] += __popc(same);
-      token[to] = t;
-      id[to] = row;
+  // half of the warps list the tokens, two pieces each; the others begin with the rows without tokens, whose stores then hide
+  // the latency of the first half's loads
+  for (int p = warp; warp < kOrderWarps / 2 && p < kOrderWarps; p += kOrderWarps / 2) {
+    const int stop = piece_start(p + 1);
+    int* next = place + p * range;
+    for (int t0 = piece_start(p); t0 < stop; t0 += 32 * AHEAD) {
+      fetch(t0, stop);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int64_t at = row[k] - first_row;
+        const bool here = at >= 0 && at < rows;
+        const unsigned active = __ballot_sync(0xffffffffu, here);
+        if (active == 0) continue;
+        if (here) {
+          const unsigned same = __match_any_sync(active, row[k]);
+          const int rank = __popc(same & ((1u << lane) - 1));
+          const int to = next[at] + rank;
+          __syncwarp(active);
+          if (rank == 0) next[at] += __popc(same);
+          token[to] = t0 + k * 32 + lane;
+          id[to] = row[k];
+        }
+        __syncwarp();
+      }
     }
-    __syncwarp();
   }
-  // rows without tokens
-  for (int r = warp; r < rows; r += kOrderWarps) {
+  // rows without tokens: words between the 16-byte boundaries, single elements around them
+  constexpr int64_t V = Num<T>::kVec;
+  for (;;) {
+    int r = 0;
+    if (lane == 0) r = atomicAdd(&next_row, 1);  // whichever warp takes it writes the same zeros
+    r = __shfl_sync(0xffffffffu, r, 0);
+    if (r >= rows) break;
     if (totals[r] != 0) continue;
     T* out = grad_weight + (first_row + r) * cols;
-    if (vec) {
-      for (int64_t c = lane * Num<T>::kVec; c < cols; c += 32 * Num<T>::kVec) st_stream(out + c, make_uint4(0, 0, 0, 0));
-    } else {
-      for (int64_t c = lane; c < cols; c += 32) out[c] = Num<T>::down(0.f);
-    }
+    const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out) / sizeof(T) % V);
+    const int64_t head = min(cols, (V - off) % V), words = (cols - head) / V, tail = head + words * V;
+    if (lane < head) out[lane] = Num<T>::down(0.f);
+    for (int64_t w = lane; w < words; w += 32) st_stream(out + head + w * V, make_uint4(0, 0, 0, 0));
+    if (tail + lane < cols) out[tail + lane] = Num<T>::down(0.f);
   }
 }
 
@@ -181,19 +212,20 @@ __device__ __forceinline__ void put_part(float* p, const float (&v)[N]) {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kSumThreads)
 embedding_sum_kernel(const T* grad, const int32_t* token, const int32_t* id, const int32_t* count,
-                     T* grad_weight, float* parts, int unit, int64_t words, int64_t cols, int64_t ldg, float scale) {
+                     T* grad_weight, float* parts, int unit, int capacity, int64_t words, int64_t cols, int64_t ldg, float scale) {
   using W = Word<T, VEC>;
   constexpr int N = W::N, AHEAD = 8;
   __shared__ int tokens[kMaxUnit], ids[kMaxUnit + 2];
   pdl_prologue();
-  const int total = *count, first = blockIdx.x * unit;
+  // all three loads at once: what lies behind the list's end is read and not used
+  const int first = blockIdx.x * unit, i = first + static_cast<int>(threadIdx.x);
+  const int mine = threadIdx.x < unit && i < capacity ? token[i] : 0;
+  const int my_id = threadIdx.x < unit + 2 && i >= 1 && i <= capacity ? id[i - 1] : -1;
+  const int total = *count;
   if (first >= total) return;
   const int n = min(unit, total - first);
-  if (threadIdx.x < n) tokens[threadIdx.x] = token[first + threadIdx.x];
-  if (threadIdx.x < n + 2) {
-    const int i = first + static_cast<int>(threadIdx.x) - 1;
-    ids[threadIdx.x] = i >= 0 && i < total ? id[i] : -1;  // with the neighbours of the unit
-  }
+  if (threadIdx.x < n) tokens[threadIdx.x] = mine;
+  if (threadIdx.x < n + 2) ids[threadIdx.x] = i <= total ? my_id : -1;  // with the neighbours of the unit
   __syncthreads();
   const int64_t w = static_cast<int64_t>(blockIdx.y) * kSumThreads + threadIdx.x;
   if (w >= words) return;
@@ -234,22 +266,104 @@ embedding_sum_kernel(const T* grad, const int32_t* token, const int32_t* id, con
   }
 }
 
-// One CTA per unit and 128 columns; it has work where a run begins in the unit and goes on in the next.
+// Adds up the parts of the runs that cross units.  A CTA looks after kJoinUnits units and 128 columns.  Each warp takes some
+// of the runs that begin in these units and go on; one of more than kLongRun parts is added up by all warps, each an equal
+// share of its parts, the shares in warp order.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinColumns = 128;
+constexpr int kJoinUnits = 32, kLongRun = 64;
+
+// the last unit that the run of unit `begin` reaches: 32 units probed at a time, next to it first
+__device__ __forceinline__ int last_unit(const int32_t* id, int run, int begin, int units, int unit) {
+  const int lane = threadIdx.x & 31;
+  int low = begin + 1, high = units - 1, step = 1;
+  while (low < high) {
+    const int64_t probe = low + static_cast<int64_t>(lane + 1) * step;
+    const int reached = __popc(__ballot_sync(0xffffffffu, probe <= high && id[min(probe, static_cast<int64_t>(high)) * unit] == run));
+    low += reached * step;
+    if (reached < 32) high = min(high, low + step - 1);
+    step = max(1, (high - low + 31) / 32);
+  }
+  return low;
+}
+
+__device__ __forceinline__ float4 add_parts(const float* parts, int begin, int from, int to, int64_t cols, int64_t c) {
+  const bool words = cols % 4 == 0;  // of four columns
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = from; i < to; ++i) {
+    const float* part = parts + (static_cast<int64_t>(begin + i) * 2 + (i == 0 ? 1 : 0)) * cols + c;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (words && c < cols) {
+      v = *reinterpret_cast<const float4*>(part);
+    } else {
+      if (c < cols) v.x = part[0];
+      if (c + 1 < cols) v.y = part[1];
+      if (c + 2 < cols) v.z = part[2];
+      if (c + 3 < cols) v.w = part[3];
+    }
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  }
+  return sum;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(128)
-embedding_join_kernel(const int32_t* id, const int32_t* count, const float* parts, T* grad_weight,
-                      int unit, int64_t cols, float scale) {
+__global__ void __launch_bounds__(kJoinThreads)
+embedding_join_kernel(const int32_t* id, const int32_t* count, const float* parts, T* grad_weight, int unit, int64_t cols, float scale) {
+  __shared__ int long_begin[kJoinUnits], long_parts[kJoinUnits];
+  __shared__ int found;
+  __shared__ float4 share[kJoinWarps][32];
+  if (threadIdx.x == 0) found = 0;
   pdl_prologue();
-  const int total = *count;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * unit, next = first + unit;
-  if (next >= total) return;
-  const int run = id[next - 1];
-  if (id[next] != run || (first > 0 && id[first - 1] == run)) return;  // no run crosses, or an earlier unit has its beginning
-  const int64_t c = static_cast<int64_t>(blockIdx.y) * 128 + threadIdx.x;
-  if (c >= cols) return;
-  float sum = parts[(static_cast<int64_t>(blockIdx.x) * 2 + 1) * cols + c];
-  for (int64_t u = blockIdx.x + 1; u * unit < total && id[u * unit] == run; ++u) sum += parts[u * 2 * cols + c];
-  grad_weight[run * cols + c] = Num<T>::down(sum * scale);
+  const int total = *count, units = (total + unit - 1) / unit;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int u0 = blockIdx.x * kJoinUnits;
+  if (u0 + 1 >= units) return;
+  const int64_t c = static_cast<int64_t>(blockIdx.y) * kJoinColumns + lane * 4;
+  bool begins = false;  // a run begins in this lane's unit and goes on in the next
+  int my_run = 0;
+  if (u0 + lane + 1 < units) {
+    const int64_t first = static_cast<int64_t>(u0 + lane) * unit;
+    my_run = id[first + unit - 1];
+    const int behind = id[first + unit], start = id[first], before = first == 0 ? -1 : id[first - 1];
+    begins = behind == my_run && (start != my_run || before != my_run);
+  }
+  __syncthreads();  // `found` is zero
+  unsigned todo = __ballot_sync(0xffffffffu, begins);
+  for (int k = 0; todo != 0; ++k, todo &= todo - 1) {
+    if (k % kJoinWarps != warp) continue;
+    const int at = __ffs(todo) - 1, begin = u0 + at, run = __shfl_sync(0xffffffffu, my_run, at);
+    const int n = last_unit(id, run, begin, units, unit) - begin + 1;  // parts: the second of unit `begin`, the first of the others
+    if (n > kLongRun) {
+      if (lane == 0) {
+        const int slot = atomicAdd(&found, 1);  // in any order: the runs do not meet
+        long_begin[slot] = begin;
+        long_parts[slot] = n;
+      }
+      continue;
+    }
+    const float4 sum = add_parts(parts, begin, 0, n, cols, c);
+    T* out = grad_weight + run * cols + c;
+    if (c < cols) out[0] = Num<T>::down(sum.x * scale);
+    if (c + 1 < cols) out[1] = Num<T>::down(sum.y * scale);
+    if (c + 2 < cols) out[2] = Num<T>::down(sum.z * scale);
+    if (c + 3 < cols) out[3] = Num<T>::down(sum.w * scale);
+  }
+  __syncthreads();
+  const int runs = found;
+  for (int k = 0; k < runs; ++k) {
+    const int begin = long_begin[k], n = long_parts[k], run = id[static_cast<int64_t>(begin) * unit + unit - 1];
+    const float4 sum = add_parts(parts, begin, static_cast<int>(static_cast<int64_t>(n) * warp / kJoinWarps), static_cast<int>(static_cast<int64_t>(n) * (warp + 1) / kJoinWarps), cols, c);
+    __syncthreads();  // the run before has been read
+    share[warp][lane] = sum;
+    __syncthreads();
+    const int64_t column = static_cast<int64_t>(blockIdx.y) * kJoinColumns + threadIdx.x;
+    if (threadIdx.x < kJoinColumns && column < cols) {
+      float all = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) all += reinterpret_cast<const float*>(share[w])[threadIdx.x];
+      grad_weight[run * cols + column] = Num<T>::down(all * scale);
+    }
+  }
 }
 
 struct Scratch {
@@ -297,20 +411,20 @@ int run_backward(const void* grad_out, const void* ids, void* grad_weight, int64
     return fail(B200_ERR_LAUNCH, "embedding_order_kernel: %s", cudaGetErrorString(cudaGetLastError()));
   const int pad = padding >= 0 && padding < vocab ? static_cast<int>(padding) : -1;
   launch(order, static_cast<unsigned>(ceil_div(vocab, range)), kOrderThreads, smem, st, static_cast<const I*>(ids), static_cast<int>(tokens), vocab, pad,
-         range, s.token, s.id, s.count, out, cols, cols % V == 0 && aligned(out, 16));
+         range, s.token, s.id, s.count, out, cols);
   if (int rc = after_launch("embedding_order_kernel")) return rc;
   if (tokens == 0) return B200_OK;
   const int unit = unit_length(tokens);
   const int64_t words = vec ? cols / V : cols, units = ceil_div(tokens, unit);
   const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(words, kSumThreads)));
   if (vec)
-    launch(embedding_sum_kernel<T, true>, grid, kSumThreads, 0, st, g, s.token, s.id, s.count, out, s.parts, unit, words, cols, ldg, scale);
+    launch(embedding_sum_kernel<T, true>, grid, kSumThreads, 0, st, g, s.token, s.id, s.count, out, s.parts, unit, static_cast<int>(tokens), words, cols, ldg, scale);
   else
-    launch(embedding_sum_kernel<T, false>, grid, kSumThreads, 0, st, g, s.token, s.id, s.count, out, s.parts, unit, words, cols, ldg, scale);
+    launch(embedding_sum_kernel<T, false>, grid, kSumThreads, 0, st, g, s.token, s.id, s.count, out, s.parts, unit, static_cast<int>(tokens), words, cols, ldg, scale);
   if (int rc = after_launch("embedding_sum_kernel")) return rc;
   if (units > 1) {
-    const dim3 joins(static_cast<unsigned>(units - 1), static_cast<unsigned>(ceil_div(cols, 128)));
-    launch(embedding_join_kernel<T>, joins, 128, 0, st, s.id, s.count, static_cast<const float*>(s.parts), out, unit, cols, scale);
+    const dim3 joins(static_cast<unsigned>(ceil_div(units - 1, kJoinUnits)), static_cast<unsigned>(ceil_div(cols, kJoinColumns)));
+    launch(embedding_join_kernel<T>, joins, kJoinThreads, 0, st, s.id, s.count, static_cast<const float*>(s.parts), out, unit, cols, scale);
     return after_launch("embedding_join_kernel");
   }
   return B200_OK;
