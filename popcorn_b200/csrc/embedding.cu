@@ -6,24 +6,28 @@
 // Bound by HBM: grad_out read once, every row of the table written once.  Three launches:
 //   1. order: CTA c owns a range of at most 1024 rows of the table.  It goes over all ids, counts those below its range
 //      (that is where its part of the sorted list starts) and those of each of its rows, and lists its tokens by (id, t).
-//      No CTA waits for another.  Rows that no token has are zeroed here.
+//      No CTA waits for another.  Meanwhile four of its warps begin to zero the rows that no token has.
 //   2. sums: the sorted list is cut into units of equal length, so that a frequent token is spread over many CTAs.  A run
 //      of equal ids inside a unit goes straight to its row; the parts of one that crosses units go to scratch in fp32.
-//   3. join: adds up the parts of such runs, in order.
+//   3. join: adds up the parts of such runs, in order, beside the zeroing of the rest of the rows that no token has.
+// The zeros are most of what is written for a large table; spread over the first and third launch they hide the latency
+// of the listing and of the joining (65536 tokens, fp16 [131072, 4096]: 278 us with all of them in the first, ZEROS with this).
 // No pointer is __restrict__: the second and third kernel begin with loads of what the kernel before them wrote (see ld_kept).
 // No atomics on values and a fixed order of every sum: the same inputs give the same bits.
 #include <algorithm>
 
 #include "common.cuh"
+#include "tma.cuh"
 
 namespace b200 {
 namespace {
 
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
+constexpr int kListWarps = kOrderWarps - 4;  // list the tokens, one piece of them each; the others zero rows meanwhile
 constexpr int kMaxRange = 1024;   // rows of the table per CTA of the order kernel
 constexpr int kSumThreads = 128;  // one load of each row per thread: a tile of columns
-constexpr int kMaxUnit = 32;      // sorted tokens per unit
+constexpr int kMaxUnit = 64;      // sorted tokens per unit
 
 template <typename T, bool VEC>
 struct Word;
@@ -78,27 +82,61 @@ embedding_kernel(const I* ids, const T* weight, T* out, int64_t tokens, int64_t 
   }
 }
 
+// Zeroing of table rows by bulk copies out of a zeroed piece of shared memory, eight threads a row and four rows a warp:
+// the copy engine keeps the memory busy by itself (16-byte stores of eight warps per SM reached 3.6 TB/s).
+constexpr int kZeroBytes = 1024, kZeroLanes = 8, kZeroRows = 32 / kZeroLanes;
+struct Zeros {
+  uint4 words[kZeroBytes / 16];
+  __device__ __forceinline__ void clear(int threads) {
+    for (int i = threadIdx.x; i < kZeroBytes / 16; i += threads) words[i] = make_uint4(0, 0, 0, 0);
+    fence_async_smem();  // before the barrier behind which the copies are issued
+  }
+};
+// this thread's copies of a row: what lies between 16-byte boundaries; single elements around it
+template <typename T>
+__device__ __forceinline__ void zero_row(const Zeros& zeros, T* out, int64_t cols) {
+  const int part = threadIdx.x % kZeroLanes;
+  unsigned char* begin = reinterpret_cast<unsigned char*>(out);
+  unsigned char* end = reinterpret_cast<unsigned char*>(out + cols);
+  unsigned char* from = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(begin) + 15) & ~static_cast<uintptr_t>(15));
+  unsigned char* to = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(end) & ~static_cast<uintptr_t>(15));
+  if (from >= to) from = to = end;
+  for (T* p = out + part; reinterpret_cast<unsigned char*>(p) < from; p += kZeroLanes) *p = Num<T>::down(0.f);
+  for (T* p = reinterpret_cast<T*>(to) + part; reinterpret_cast<unsigned char*>(p) < end; p += kZeroLanes) *p = Num<T>::down(0.f);
+  if (cols * sizeof(T) % 128 != 0) {
+    for (from += part * 16; from < to; from += kZeroLanes * 16) st_stream(from, make_uint4(0, 0, 0, 0));
+    return;
+  }
+  for (from += part * kZeroBytes; from < to; from += kZeroLanes * kZeroBytes)
+    bulk_store(from, zeros.words, static_cast<uint32_t>(min(static_cast<int64_t>(to - from), static_cast<int64_t>(kZeroBytes))));
+}
+
 // The tokens by (id, t): token[i] and id[i] for i < *count.
 template <typename T, typename I>
 __global__ void __launch_bounds__(kOrderThreads)
 embedding_order_kernel(const I* ids, int tokens, int64_t vocab, int padding, int range, int32_t* token,
-                       int32_t* id, int32_t* count, T* grad_weight, int64_t cols) {
+                       int32_t* id, int32_t* count, uint8_t* hit, int32_t* resume, T* grad_weight, int64_t cols) {
   constexpr int AHEAD = 8;
   extern __shared__ int place[];  // [warp][row of the range]: first the warp's tokens of the row, then where they go
   __shared__ int totals[kMaxRange];
   __shared__ int fold[kOrderWarps];
-  __shared__ int next_row;
+  __shared__ __align__(128) Zeros zeros;
+  __shared__ int next_row, listing;  // the next row to look at for zeroing; warps that are still listing
   pdl_prologue();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t first_row = static_cast<int64_t>(blockIdx.x) * range;
   const int rows = static_cast<int>(min(static_cast<int64_t>(range), vocab - first_row));
-  if (threadIdx.x == 0) next_row = 0;
-  for (int i = threadIdx.x; i < kOrderWarps * range; i += kOrderThreads) place[i] = 0;
+  if (threadIdx.x == 0) {
+    next_row = 0;
+    listing = kListWarps;
+  }
+  zeros.clear(kOrderThreads);
+  for (int i = threadIdx.x; i < kListWarps * range; i += kOrderThreads) place[i] = 0;
   __syncthreads();
   // the ids in one contiguous piece per warp, so that piece order is token order
-  const int piece = (tokens + kOrderWarps - 1) / kOrderWarps;
+  const int piece = (tokens + kListWarps - 1) / kListWarps;
   auto piece_start = [&](int p) { return static_cast<int>(min(static_cast<int64_t>(tokens), static_cast<int64_t>(p) * piece)); };
-  const int begin = piece_start(warp), end = piece_start(warp + 1);
+  const int begin = piece_start(warp), end = warp < kListWarps ? piece_start(warp + 1) : begin;
   int below = 0;
   // the rows of eight batches of a warp's tokens at a time; -1: none, also for padding
   int row[AHEAD];
@@ -131,12 +169,13 @@ embedding_order_kernel(const I* ids, int tokens, int64_t vocab, int padding, int
   int mine = 0;
   if (threadIdx.x < rows) {
 #pragma unroll 8
-    for (int w = 0; w < kOrderWarps; ++w) {
+    for (int w = 0; w < kListWarps; ++w) {
       const int n = place[w * range + threadIdx.x];
       place[w * range + threadIdx.x] = mine;
       mine += n;
     }
     totals[threadIdx.x] = mine;
+    hit[first_row + threadIdx.x] = mine != 0;
   }
   int scan = mine;
 #pragma unroll
@@ -155,17 +194,17 @@ embedding_order_kernel(const I* ids, int tokens, int64_t vocab, int padding, int
   if (threadIdx.x < rows) {
     const int at = start + before + scan - mine;
 #pragma unroll 8
-    for (int w = 0; w < kOrderWarps; ++w) place[w * range + threadIdx.x] += at;
+    for (int w = 0; w < kListWarps; ++w) place[w * range + threadIdx.x] += at;
   }
-  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *count = start + all;
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+    count[0] = start + all;
+    count[1] = 0;  // the join kernel's next row to zero
+  }
   __syncthreads();
-  // half of the warps list the tokens, two pieces each; the others begin with the rows without tokens, whose stores then hide
-  // the latency of the first half's loads
-  for (int p = warp; warp < kOrderWarps / 2 && p < kOrderWarps; p += kOrderWarps / 2) {
-    const int stop = piece_start(p + 1);
-    int* next = place + p * range;
-    for (int t0 = piece_start(p); t0 < stop; t0 += 32 * AHEAD) {
-      fetch(t0, stop);
+  if (warp < kListWarps) {
+    int* next = place + warp * range;
+    for (int t0 = begin; t0 < end; t0 += 32 * AHEAD) {
+      fetch(t0, end);
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int64_t at = row[k] - first_row;
@@ -184,22 +223,22 @@ embedding_order_kernel(const I* ids, int tokens, int64_t vocab, int padding, int
         __syncwarp();
       }
     }
+    if (lane == 0) atomicSub(&listing, 1);
+  } else {
+    for (;;) {
+      int r = rows;
+      if (lane == 0 && *static_cast<volatile int*>(&listing) > 0) r = atomicAdd(&next_row, kZeroRows);  // whichever warp takes them writes the same zeros
+      r = __shfl_sync(0xffffffffu, r, 0);
+      if (r >= rows) break;
+      r += lane / kZeroLanes;
+      if (r < rows && totals[r] == 0) zero_row(zeros, grad_weight + (first_row + r) * cols, cols);
+      bulk_commit();
+      bulk_wait_read<4>();  // no further ahead than that: the kernel ends with the list
+    }
+    bulk_wait_all<0>();
   }
-  // rows without tokens: words between the 16-byte boundaries, single elements around them
-  constexpr int64_t V = Num<T>::kVec;
-  for (;;) {
-    int r = 0;
-    if (lane == 0) r = atomicAdd(&next_row, 1);  // whichever warp takes it writes the same zeros
-    r = __shfl_sync(0xffffffffu, r, 0);
-    if (r >= rows) break;
-    if (totals[r] != 0) continue;
-    T* out = grad_weight + (first_row + r) * cols;
-    const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out) / sizeof(T) % V);
-    const int64_t head = min(cols, (V - off) % V), words = (cols - head) / V, tail = head + words * V;
-    if (lane < head) out[lane] = Num<T>::down(0.f);
-    for (int64_t w = lane; w < words; w += 32) st_stream(out + head + w * V, make_uint4(0, 0, 0, 0));
-    if (tail + lane < cols) out[tail + lane] = Num<T>::down(0.f);
-  }
+  __syncthreads();
+  if (threadIdx.x == 0) resume[blockIdx.x] = next_row;  // rows below it are done
 }
 
 template <int N>
@@ -266,11 +305,13 @@ embedding_sum_kernel(const T* grad, const int32_t* token, const int32_t* id, con
   }
 }
 
-// Adds up the parts of the runs that cross units.  A CTA looks after kJoinUnits units and 128 columns.  Each warp takes some
-// of the runs that begin in these units and go on; one of more than kLongRun parts is added up by all warps, each an equal
-// share of its parts, the shares in warp order.
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinColumns = 128;
-constexpr int kJoinUnits = 32, kLongRun = 64;
+// `fillers` of the CTAs zero the rows without tokens that the order kernel has not come to.  The others add up the parts of
+// the runs that cross units.  A CTA looks after eight units, one per warp, and 256 columns; a warp has
+// work where a run begins in its unit and goes on in the next.  A run of more than kLongRun parts is added up by all warps,
+// each an equal share of its parts, the shares in warp order.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinColumns = 256;
+constexpr int kLongRun = 32;
+constexpr int kJoinWords = kJoinColumns / 128;  // float4 of a lane: columns lane * 4 + 128 * i
 
 // the last unit that the run of unit `begin` reaches: 32 units probed at a time, next to it first
 __device__ __forceinline__ int last_unit(const int32_t* id, int run, int begin, int units, int unit) {
@@ -286,93 +327,134 @@ __device__ __forceinline__ int last_unit(const int32_t* id, int run, int begin, 
   return low;
 }
 
-__device__ __forceinline__ float4 add_parts(const float* parts, int begin, int from, int to, int64_t cols, int64_t c) {
-  const bool words = cols % 4 == 0;  // of four columns
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int i = from; i < to; ++i) {
-    const float* part = parts + (static_cast<int64_t>(begin + i) * 2 + (i == 0 ? 1 : 0)) * cols + c;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (words && c < cols) {
-      v = *reinterpret_cast<const float4*>(part);
+// sum += the four columns from c of one part, for each of the lane's words
+__device__ __forceinline__ void add_part(const float* part, int64_t cols, int64_t c0, float4 (&sum)[kJoinWords]) {
+  float4 v[kJoinWords];
+#pragma unroll
+  for (int i = 0; i < kJoinWords; ++i) {
+    const int64_t c = c0 + 128 * i;
+    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (cols % 4 == 0) {
+      if (c < cols) v[i] = *reinterpret_cast<const float4*>(part + c);
     } else {
-      if (c < cols) v.x = part[0];
-      if (c + 1 < cols) v.y = part[1];
-      if (c + 2 < cols) v.z = part[2];
-      if (c + 3 < cols) v.w = part[3];
+      if (c < cols) v[i].x = part[c];
+      if (c + 1 < cols) v[i].y = part[c + 1];
+      if (c + 2 < cols) v[i].z = part[c + 2];
+      if (c + 3 < cols) v[i].w = part[c + 3];
     }
-    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
   }
-  return sum;
+#pragma unroll
+  for (int i = 0; i < kJoinWords; ++i) sum[i].x += v[i].x, sum[i].y += v[i].y, sum[i].z += v[i].z, sum[i].w += v[i].w;
+}
+template <typename T>
+__device__ __forceinline__ void put_row(T* out, int64_t cols, int64_t c0, const float4 (&sum)[kJoinWords], float scale) {
+#pragma unroll
+  for (int i = 0; i < kJoinWords; ++i) {
+    const int64_t c = c0 + 128 * i;
+    if (c < cols) out[c] = Num<T>::down(sum[i].x * scale);
+    if (c + 1 < cols) out[c + 1] = Num<T>::down(sum[i].y * scale);
+    if (c + 2 < cols) out[c + 2] = Num<T>::down(sum[i].z * scale);
+    if (c + 3 < cols) out[c + 3] = Num<T>::down(sum[i].w * scale);
+  }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads)
-embedding_join_kernel(const int32_t* id, const int32_t* count, const float* parts, T* grad_weight, int unit, int64_t cols, float scale) {
-  __shared__ int long_begin[kJoinUnits], long_parts[kJoinUnits];
-  __shared__ int found;
-  __shared__ float4 share[kJoinWarps][32];
-  if (threadIdx.x == 0) found = 0;
+__global__ void __launch_bounds__(kJoinThreads, 4)
+embedding_join_kernel(const int32_t* id, const int32_t* count, const float* parts, T* grad_weight, int unit, int capacity, int64_t cols, float scale, int fillers,
+                      int column_tiles, const uint8_t* hit, const int32_t* resume, int* next_row, int64_t vocab, int range) {
+  __shared__ int long_parts[kJoinWarps], long_run[kJoinWarps];  // of each warp's run, 0: it was short, or there was none
+  __shared__ float4 share[kJoinWarps][kJoinWords][32];
   pdl_prologue();
-  const int total = *count, units = (total + unit - 1) / unit;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int u0 = blockIdx.x * kJoinUnits;
-  if (u0 + 1 >= units) return;
-  const int64_t c = static_cast<int64_t>(blockIdx.y) * kJoinColumns + lane * 4;
-  bool begins = false;  // a run begins in this lane's unit and goes on in the next
-  int my_run = 0;
-  if (u0 + lane + 1 < units) {
-    const int64_t first = static_cast<int64_t>(u0 + lane) * unit;
-    my_run = id[first + unit - 1];
-    const int behind = id[first + unit], start = id[first], before = first == 0 ? -1 : id[first - 1];
-    begins = behind == my_run && (start != my_run || before != my_run);
-  }
-  __syncthreads();  // `found` is zero
-  unsigned todo = __ballot_sync(0xffffffffu, begins);
-  for (int k = 0; todo != 0; ++k, todo &= todo - 1) {
-    if (k % kJoinWarps != warp) continue;
-    const int at = __ffs(todo) - 1, begin = u0 + at, run = __shfl_sync(0xffffffffu, my_run, at);
-    const int n = last_unit(id, run, begin, units, unit) - begin + 1;  // parts: the second of unit `begin`, the first of the others
-    if (n > kLongRun) {
-      if (lane == 0) {
-        const int slot = atomicAdd(&found, 1);  // in any order: the runs do not meet
-        long_begin[slot] = begin;
-        long_parts[slot] = n;
+  // fillers and joiners take turns as long as there are both: an SM gets some of either
+  const int joiners = gridDim.x - fillers, turns = 2 * min(fillers, joiners), b = blockIdx.x;
+  const bool filler = b < turns ? b % 2 == 0 : fillers > joiners;
+  if (filler) {  // eight rows of the table at a time and warp
+    __shared__ __align__(128) Zeros zeros;
+    zeros.clear(kJoinThreads);
+    __syncthreads();
+    for (;;) {
+      int v0 = 0;
+      if (lane == 0) v0 = atomicAdd(next_row, 2 * kZeroRows);  // whichever warp takes them writes the same zeros
+      v0 = __shfl_sync(0xffffffffu, v0, 0);
+      if (v0 >= vocab) break;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int64_t v = v0 + k * kZeroRows + lane / kZeroLanes;
+        if (v < vocab && hit[v] == 0 && v % range >= resume[v / range]) zero_row(zeros, grad_weight + v * cols, cols);
       }
-      continue;
+      bulk_commit();
+      bulk_wait_read<4>();
     }
-    const float4 sum = add_parts(parts, begin, 0, n, cols, c);
-    T* out = grad_weight + run * cols + c;
-    if (c < cols) out[0] = Num<T>::down(sum.x * scale);
-    if (c + 1 < cols) out[1] = Num<T>::down(sum.y * scale);
-    if (c + 2 < cols) out[2] = Num<T>::down(sum.z * scale);
-    if (c + 3 < cols) out[3] = Num<T>::down(sum.w * scale);
+    bulk_wait_all<0>();
+    return;
+  }
+  const int joiner = b < turns ? b / 2 : b - fillers, block = joiner / column_tiles;
+  const int u = block * kJoinWarps + warp;
+  const int64_t first = static_cast<int64_t>(u) * unit, c0 = static_cast<int64_t>(joiner % column_tiles) * kJoinColumns + lane * 4;
+  // the ids around the unit's two ends and the length of the list, in one round of loads
+  const int64_t at = lane == 0 ? first - 1 : lane == 1 ? first : first + unit + lane - 3;
+  const int mine = lane < 4 && at >= 0 && at < capacity ? id[at] : -1;
+  const int total = *count, units = (total + unit - 1) / unit;
+  const int before = __shfl_sync(0xffffffffu, mine, 0), start = __shfl_sync(0xffffffffu, mine, 1), run = __shfl_sync(0xffffffffu, mine, 2), behind = __shfl_sync(0xffffffffu, mine, 3);
+  int n = 0;  // parts: the second of unit u, the first of the units behind it
+  if (first + unit < total && behind == run && (start != run || before != run)) {
+    n = last_unit(id, run, u, units, unit) - u + 1;
+    if (n <= kLongRun) {
+      float4 sum[kJoinWords] = {};
+      add_part(parts + (static_cast<int64_t>(u) * 2 + 1) * cols, cols, c0, sum);
+#pragma unroll 4
+      for (int i = 1; i < n; ++i) add_part(parts + static_cast<int64_t>(u + i) * 2 * cols, cols, c0, sum);
+      put_row(grad_weight + run * cols, cols, c0, sum, scale);
+    }
+  }
+  if (lane == 0) {
+    long_parts[warp] = n > kLongRun ? n : 0;
+    long_run[warp] = run;
   }
   __syncthreads();
-  const int runs = found;
-  for (int k = 0; k < runs; ++k) {
-    const int begin = long_begin[k], n = long_parts[k], run = id[static_cast<int64_t>(begin) * unit + unit - 1];
-    const float4 sum = add_parts(parts, begin, static_cast<int>(static_cast<int64_t>(n) * warp / kJoinWarps), static_cast<int>(static_cast<int64_t>(n) * (warp + 1) / kJoinWarps), cols, c);
-    __syncthreads();  // the run before has been read
-    share[warp][lane] = sum;
-    __syncthreads();
-    const int64_t column = static_cast<int64_t>(blockIdx.y) * kJoinColumns + threadIdx.x;
-    if (threadIdx.x < kJoinColumns && column < cols) {
-      float all = 0.f;
+  for (int k = 0; k < kJoinWarps; ++k) {
+    n = long_parts[k];
+    if (n == 0) continue;
+    const int64_t begin = static_cast<int64_t>(block) * kJoinWarps + k;
+    float4 sum[kJoinWords] = {};
+#pragma unroll 4
+    for (int i = static_cast<int>(static_cast<int64_t>(n) * warp / kJoinWarps); i < static_cast<int>(static_cast<int64_t>(n) * (warp + 1) / kJoinWarps); ++i)
+      add_part(parts + ((begin + i) * 2 + (i == 0 ? 1 : 0)) * cols, cols, c0, sum);
 #pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) all += reinterpret_cast<const float*>(share[w])[threadIdx.x];
-      grad_weight[run * cols + column] = Num<T>::down(all * scale);
+    for (int i = 0; i < kJoinWords; ++i) share[warp][i][lane] = sum[i];
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int i = 0; i < kJoinWords; ++i) {
+        sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < kJoinWarps; ++w) {
+          const float4 v = share[w][i][lane];
+          sum[i].x += v.x, sum[i].y += v.y, sum[i].z += v.z, sum[i].w += v.w;
+        }
+      }
+      put_row(grad_weight + long_run[k] * cols, cols, c0, sum, scale);
     }
+    __syncthreads();
   }
 }
 
 struct Scratch {
-  int32_t *token, *id, *count;
+  int32_t *token, *id, *count, *resume;
+  uint8_t* hit;
   float* parts;
 };
-int unit_length(int64_t tokens) { return tokens >= 8192 ? kMaxUnit : 8; }
-size_t scratch_layout(int64_t tokens, int64_t cols, char* base, Scratch* out) {
-  const int64_t units = ceil_div(tokens, unit_length(tokens));
+// Sorted tokens per unit: long units mean few runs that cross them, as long as some 700 CTAs are left.
+int unit_length(int64_t tokens, int64_t cols) {
+  int unit = 8;
+  while (unit < kMaxUnit && tokens * ceil_div(cols, 512) / (2 * unit) >= 700) unit *= 2;
+  return unit;
+}
+// CTAs of the order kernel: one per SM, or as many as ranges of kMaxRange rows take.
+constexpr int kMaxOrderCtas = 512;
+int64_t order_ctas(int64_t vocab) { return std::max<int64_t>(std::min(sm_count(), kMaxOrderCtas), ceil_div(vocab, kMaxRange)); }
+size_t scratch_layout(int64_t tokens, int64_t vocab, int64_t cols, char* base, Scratch* out) {
+  const int64_t units = ceil_div(tokens, unit_length(tokens, cols));
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -380,7 +462,9 @@ size_t scratch_layout(int64_t tokens, int64_t cols, char* base, Scratch* out) {
     return base + here;
   };
   Scratch s;
-  s.count = reinterpret_cast<int32_t*>(take(4));
+  s.count = reinterpret_cast<int32_t*>(take(8));
+  s.resume = reinterpret_cast<int32_t*>(take(static_cast<size_t>(std::max<int64_t>(kMaxOrderCtas, ceil_div(vocab, kMaxRange))) * 4));
+  s.hit = reinterpret_cast<uint8_t*>(take(static_cast<size_t>(vocab)));
   s.token = reinterpret_cast<int32_t*>(take(static_cast<size_t>(tokens) * 4));
   s.id = reinterpret_cast<int32_t*>(take(static_cast<size_t>(tokens) * 4));
   s.parts = reinterpret_cast<float*>(take(static_cast<size_t>(units) * 2 * static_cast<size_t>(cols) * 4));
@@ -403,31 +487,30 @@ int run_backward(const void* grad_out, const void* ids, void* grad_weight, int64
   const T* g = static_cast<const T*>(grad_out);
   T* out = static_cast<T*>(grad_weight);
   const bool vec = cols % V == 0 && ldg % V == 0 && aligned(g, 16) && aligned(out, 16);
-  const int64_t ctas = std::max<int64_t>(sm_count(), ceil_div(vocab, kMaxRange));
-  const int range = static_cast<int>(ceil_div(vocab, ctas));
-  const size_t smem = static_cast<size_t>(range) * kOrderWarps * sizeof(int);
+  const int range = static_cast<int>(ceil_div(vocab, order_ctas(vocab)));
+  const size_t smem = static_cast<size_t>(range) * kListWarps * sizeof(int);
   auto order = embedding_order_kernel<T, I>;
   if (cudaFuncSetAttribute(order, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
     return fail(B200_ERR_LAUNCH, "embedding_order_kernel: %s", cudaGetErrorString(cudaGetLastError()));
   const int pad = padding >= 0 && padding < vocab ? static_cast<int>(padding) : -1;
   launch(order, static_cast<unsigned>(ceil_div(vocab, range)), kOrderThreads, smem, st, static_cast<const I*>(ids), static_cast<int>(tokens), vocab, pad,
-         range, s.token, s.id, s.count, out, cols);
+         range, s.token, s.id, s.count, s.hit, s.resume, out, cols);
   if (int rc = after_launch("embedding_order_kernel")) return rc;
-  if (tokens == 0) return B200_OK;
-  const int unit = unit_length(tokens);
+  const int unit = unit_length(tokens, cols);
   const int64_t words = vec ? cols / V : cols, units = ceil_div(tokens, unit);
-  const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(words, kSumThreads)));
-  if (vec)
-    launch(embedding_sum_kernel<T, true>, grid, kSumThreads, 0, st, g, s.token, s.id, s.count, out, s.parts, unit, static_cast<int>(tokens), words, cols, ldg, scale);
-  else
-    launch(embedding_sum_kernel<T, false>, grid, kSumThreads, 0, st, g, s.token, s.id, s.count, out, s.parts, unit, static_cast<int>(tokens), words, cols, ldg, scale);
-  if (int rc = after_launch("embedding_sum_kernel")) return rc;
-  if (units > 1) {
-    const dim3 joins(static_cast<unsigned>(ceil_div(units - 1, kJoinUnits)), static_cast<unsigned>(ceil_div(cols, kJoinColumns)));
-    launch(embedding_join_kernel<T>, joins, kJoinThreads, 0, st, s.id, s.count, static_cast<const float*>(s.parts), out, unit, cols, scale);
-    return after_launch("embedding_join_kernel");
+  if (tokens > 0) {
+    const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(words, kSumThreads)));
+    if (vec)
+      launch(embedding_sum_kernel<T, true>, grid, kSumThreads, 0, st, g, s.token, s.id, s.count, out, s.parts, unit, static_cast<int>(tokens), words, cols, ldg, scale);
+    else
+      launch(embedding_sum_kernel<T, false>, grid, kSumThreads, 0, st, g, s.token, s.id, s.count, out, s.parts, unit, static_cast<int>(tokens), words, cols, ldg, scale);
+    if (int rc = after_launch("embedding_sum_kernel")) return rc;
   }
-  return B200_OK;
+  const int fillers = 4 * sm_count();  // every place
+  const int64_t tiles = ceil_div(cols, kJoinColumns), joins = units > 1 ? ceil_div(units - 1, kJoinWarps) * tiles : 0;
+  launch(embedding_join_kernel<T>, static_cast<unsigned>(fillers + joins), kJoinThreads, 0, st, s.id, s.count, static_cast<const float*>(s.parts), out, unit,
+         static_cast<int>(tokens), cols, scale, fillers, static_cast<int>(tiles), static_cast<const uint8_t*>(s.hit), static_cast<const int32_t*>(s.resume), s.count + 1, vocab, range);
+  return after_launch("embedding_join_kernel");
 }
 
 }  // namespace
@@ -470,7 +553,7 @@ extern "C" int b200_embedding(const void* ids, const void* weight, void* out, in
 extern "C" int b200_embedding_backward_scratch_bytes(int64_t tokens, int64_t vocab, int64_t cols, size_t* bytes) {
   B200_REQUIRE_PTR(bytes);
   if (int rc = check_sizes(__func__, tokens, vocab, cols, B200_F32)) return rc;
-  *bytes = scratch_layout(tokens, cols, nullptr, nullptr);
+  *bytes = scratch_layout(tokens, vocab, cols, nullptr, nullptr);
   return B200_OK;
 }
 
@@ -491,7 +574,7 @@ extern "C" int b200_embedding_backward(const void* grad_out, const void* ids, vo
     return fail(B200_ERR_ALIGNMENT, "%s: pointer not aligned to its element size", __func__);
   if (int rc = check_device()) return rc;
   Scratch s;
-  const size_t need = scratch_layout(tokens, cols, static_cast<char*>(scratch), &s);
+  const size_t need = scratch_layout(tokens, vocab, cols, static_cast<char*>(scratch), &s);
   if (scratch_bytes < need || !aligned(scratch, 16))
     return fail(B200_ERR_SCRATCH, "%s: scratch needs %zu bytes, 16-byte aligned (got %zu)", __func__, need, scratch_bytes);
   const float sc = static_cast<float>(scale);
