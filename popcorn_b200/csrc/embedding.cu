@@ -6,12 +6,12 @@
 // Bound by HBM: grad_out read once, every row of the table written once.  Three launches:
 //   1. order: CTA c owns a range of at most 1024 rows of the table.  It goes over all ids, counts those below its range
 //      (that is where its part of the sorted list starts) and those of each of its rows, and lists its tokens by (id, t).
-//      No CTA waits for another.  Meanwhile four of its warps begin to zero the rows that no token has.
+//      No CTA waits for another.  Meanwhile eight of its warps begin to zero the rows that no token has.
 //   2. sums: the sorted list is cut into units of equal length, so that a frequent token is spread over many CTAs.  A run
 //      of equal ids inside a unit goes straight to its row; the parts of one that crosses units go to scratch in fp32.
 //   3. join: adds up the parts of such runs, in order, beside the zeroing of the rest of the rows that no token has.
 // The zeros are most of what is written for a large table; spread over the first and third launch they hide the latency
-// of the listing and of the joining (65536 tokens, fp16 [131072, 4096]: 278 us with all of them in the first, ZEROS with this).
+// of the listing and of the joining (65536 tokens, fp16 [131072, 4096]: 278 us with all of them in the first, 258 with this).
 // No pointer is __restrict__: the second and third kernel begin with loads of what the kernel before them wrote (see ld_kept).
 // No atomics on values and a fixed order of every sum: the same inputs give the same bits.
 #include <algorithm>
@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
-constexpr int kListWarps = kOrderWarps - 4;  // list the tokens, one piece of them each; the others zero rows meanwhile
+constexpr int kListWarps = kOrderWarps - 8;  // list the tokens, one piece of them each; the others zero rows meanwhile
 constexpr int kMaxRange = 1024;   // rows of the table per CTA of the order kernel
 constexpr int kSumThreads = 128;  // one load of each row per thread: a tile of columns
 constexpr int kMaxUnit = 64;      // sorted tokens per unit
@@ -359,17 +359,15 @@ __device__ __forceinline__ void put_row(T* out, int64_t cols, int64_t c0, const 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads, 4)
+__global__ void __launch_bounds__(kJoinThreads, 3)
 embedding_join_kernel(const int32_t* id, const int32_t* count, const float* parts, T* grad_weight, int unit, int capacity, int64_t cols, float scale, int fillers,
                       int column_tiles, const uint8_t* hit, const int32_t* resume, int* next_row, int64_t vocab, int range) {
   __shared__ int long_parts[kJoinWarps], long_run[kJoinWarps];  // of each warp's run, 0: it was short, or there was none
   __shared__ float4 share[kJoinWarps][kJoinWords][32];
   pdl_prologue();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // fillers and joiners take turns as long as there are both: an SM gets some of either
-  const int joiners = gridDim.x - fillers, turns = 2 * min(fillers, joiners), b = blockIdx.x;
-  const bool filler = b < turns ? b % 2 == 0 : fillers > joiners;
-  if (filler) {  // eight rows of the table at a time and warp
+  const int b = blockIdx.x;
+  if (b < fillers) {  // two of an SM's three places: eight rows of the table at a time and warp
     __shared__ __align__(128) Zeros zeros;
     zeros.clear(kJoinThreads);
     __syncthreads();
@@ -389,7 +387,7 @@ embedding_join_kernel(const int32_t* id, const int32_t* count, const float* part
     bulk_wait_all<0>();
     return;
   }
-  const int joiner = b < turns ? b / 2 : b - fillers, block = joiner / column_tiles;
+  const int joiner = b - fillers, block = joiner / column_tiles;
   const int u = block * kJoinWarps + warp;
   const int64_t first = static_cast<int64_t>(u) * unit, c0 = static_cast<int64_t>(joiner % column_tiles) * kJoinColumns + lane * 4;
   // the ids around the unit's two ends and the length of the list, in one round of loads
@@ -506,7 +504,7 @@ int run_backward(const void* grad_out, const void* ids, void* grad_weight, int64
       launch(embedding_sum_kernel<T, false>, grid, kSumThreads, 0, st, g, s.token, s.id, s.count, out, s.parts, unit, static_cast<int>(tokens), words, cols, ldg, scale);
     if (int rc = after_launch("embedding_sum_kernel")) return rc;
   }
-  const int fillers = 4 * sm_count();  // every place
+  const int fillers = 2 * sm_count();
   const int64_t tiles = ceil_div(cols, kJoinColumns), joins = units > 1 ? ceil_div(units - 1, kJoinWarps) * tiles : 0;
   launch(embedding_join_kernel<T>, static_cast<unsigned>(fillers + joins), kJoinThreads, 0, st, s.id, s.count, static_cast<const float*>(s.parts), out, unit,
          static_cast<int>(tokens), cols, scale, fillers, static_cast<int>(tiles), static_cast<const uint8_t*>(s.hit), static_cast<const int32_t*>(s.resume), s.count + 1, vocab, range);
