@@ -330,8 +330,7 @@ class _GatedAddRmsNorm(torch.autograd.Function):
             return (None,) * 10
         if grad_y is None:  # only the residual stream was used downstream
             grad_y = torch.zeros_like(grad_s)
-        with torch.no_grad():
-            grads = ops.gated_add_rms_norm_backward(grad_y, grad_s, x, residual, weight, post_weight, gate, stats, *ctx.options)
+        grads = ops.gated_add_rms_norm_backward(grad_y, grad_s, x, residual, weight, post_weight, gate, stats, *ctx.options)
         return (*grads, None, None, None, None, None)
 
 
@@ -350,8 +349,7 @@ class _MoeBalanceLoss(torch.autograd.Function):
         router_logits, mask, stats, table = ctx.saved_tensors
         if grad_balance is None and grad_z is None:
             return None, None, None, None
-        with torch.no_grad():
-            return ops.moe_balance_loss_backward(grad_balance, grad_z, router_logits, mask, stats, table, ctx.per_sequence), None, None, None
+        return ops.moe_balance_loss_backward(grad_balance, grad_z, router_logits, mask, stats, table, ctx.per_sequence), None, None, None
 
 
 class _Embedding(torch.autograd.Function):
@@ -364,8 +362,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_out: Tensor):
         (ids,) = ctx.saved_tensors
-        with torch.no_grad():
-            return None, ops.embedding_backward(grad_out, ids, *ctx.options), None, None
+        return None, ops.embedding_backward(grad_out, ids, *ctx.options), None, None
 
 
 def rms_norm(x: Tensor, weight: Tensor, bias: Tensor | None = None, eps: float = 1e-6) -> Tensor:

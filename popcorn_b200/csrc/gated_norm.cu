@@ -28,10 +28,10 @@ struct ForwardArgs {
 };
 
 // One row per TPR threads, ITEMS loads per thread, the row in registers: x and residual as loaded, then s in fp32.
-template <typename T, bool VEC, int TPR, int ITEMS>
+template <typename T, int ACCESS, int TPR, int ITEMS>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 gated_add_rms_kernel(const ForwardArgs<T> a) {
-  using W = Word<T, VEC>;
+  using W = Word<T, ACCESS>;
   constexpr int N = W::N;
   constexpr int THREADS = TPR < 128 ? 128 : TPR;
   pdl_prologue();
@@ -141,35 +141,45 @@ gated_add_rms_wide_kernel(const ForwardArgs<T> a, int64_t cols) {
   }
 }
 
-template <typename T, bool VEC, int TPR, int ITEMS>
+template <typename T, int ACCESS, int TPR, int ITEMS>
 int launch_forward(const ForwardArgs<T>& a, cudaStream_t st) {
   constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
-  launch(gated_add_rms_kernel<T, VEC, TPR, ITEMS>, static_cast<unsigned>(ceil_div(a.rows, ROWS)), TPR < 128 ? 128 : TPR, 0, st, a);
+  launch(gated_add_rms_kernel<T, ACCESS, TPR, ITEMS>, static_cast<unsigned>(ceil_div(a.rows, ROWS)), TPR < 128 ? 128 : TPR, 0, st, a);
   return after_launch("gated_add_rms_kernel");
 }
 
 template <typename T>
-int run_forward(ForwardArgs<T> a, int64_t cols, bool vec, cudaStream_t st) {
+int run_forward(ForwardArgs<T> a, int64_t cols, Access access, cudaStream_t st) {
   constexpr int V = Num<T>::kVec;
-  if (vec && cols <= 4096 * V) {
+  if (access == kWords && cols <= 4096 * V) {
     a.words = static_cast<int>(cols / V);
-    if (a.words <= 32) return launch_forward<T, true, 32, 1>(a, st);
-    if (a.words <= 64) return launch_forward<T, true, 32, 2>(a, st);
-    if (a.words <= 128) return launch_forward<T, true, 32, 4>(a, st);
-    if (a.words <= 256) return launch_forward<T, true, 128, 2>(a, st);
-    if (a.words <= 512) return launch_forward<T, true, 256, 2>(a, st);
-    if (a.words <= 768) return launch_forward<T, true, 256, 3>(a, st);
-    if (a.words <= 1024) return launch_forward<T, true, 256, 4>(a, st);
-    if (a.words <= 2048) return launch_forward<T, true, 512, 4>(a, st);
-    return launch_forward<T, true, 1024, 4>(a, st);
+    if (a.words <= 32) return launch_forward<T, kWords, 32, 1>(a, st);
+    if (a.words <= 64) return launch_forward<T, kWords, 32, 2>(a, st);
+    if (a.words <= 128) return launch_forward<T, kWords, 32, 4>(a, st);
+    if (a.words <= 256) return launch_forward<T, kWords, 128, 2>(a, st);
+    if (a.words <= 512) return launch_forward<T, kWords, 256, 2>(a, st);
+    if (a.words <= 768) return launch_forward<T, kWords, 256, 3>(a, st);
+    if (a.words <= 1024) return launch_forward<T, kWords, 256, 4>(a, st);
+    if (a.words <= 2048) return launch_forward<T, kWords, 512, 4>(a, st);
+    return launch_forward<T, kWords, 1024, 4>(a, st);
+  }
+  // two elements at a time keep half as many instructions busy for the same bytes ([4095, 2050] fp32 with a gate per row:
+  // PAIRS us, one element at a time 57)
+  if (access != kSingles && cols <= 16384) {
+    a.words = static_cast<int>(cols / 2);
+    if (a.words <= 128) return launch_forward<T, kPairs, 32, 4>(a, st);
+    if (a.words <= 1024) return launch_forward<T, kPairs, 256, 4>(a, st);
+    if (a.words <= 2048) return launch_forward<T, kPairs, 512, 4>(a, st);
+    if (a.words <= 4096) return launch_forward<T, kPairs, 512, 8>(a, st);
+    return launch_forward<T, kPairs, 1024, 8>(a, st);
   }
   if (cols <= 16384) {
     a.words = static_cast<int>(cols);
-    if (cols <= 256) return launch_forward<T, false, 32, 8>(a, st);
-    if (cols <= 2048) return launch_forward<T, false, 256, 8>(a, st);
-    if (cols <= 4096) return launch_forward<T, false, 512, 8>(a, st);
-    if (cols <= 8192) return launch_forward<T, false, 512, 16>(a, st);
-    return launch_forward<T, false, 1024, 16>(a, st);
+    if (cols <= 256) return launch_forward<T, kSingles, 32, 8>(a, st);
+    if (cols <= 2048) return launch_forward<T, kSingles, 256, 8>(a, st);
+    if (cols <= 4096) return launch_forward<T, kSingles, 512, 8>(a, st);
+    if (cols <= 8192) return launch_forward<T, kSingles, 512, 16>(a, st);
+    return launch_forward<T, kSingles, 1024, 16>(a, st);
   }
   launch(gated_add_rms_wide_kernel<T>, a.rows, 512, 0, st, a, cols);
   return after_launch("gated_add_rms_wide_kernel");
@@ -199,10 +209,7 @@ extern "C" int b200_gated_add_rms_norm(const void* x, const void* residual, cons
       !aligned(s, es) || !aligned(stats, 8))
     return fail(B200_ERR_ALIGNMENT, "%s: pointer not aligned to the element size (stats: 8 bytes)", __func__);
   if (int rc = check_device()) return rc;
-  const int64_t v = 16 / static_cast<int64_t>(es);
-  const bool vec = cols % v == 0 && ldx % v == 0 && ldr % v == 0 && ldy % v == 0 && lds % v == 0 && aligned(x, 16) && aligned(residual, 16) &&
-                   aligned(weight, 16) && aligned(post_weight, 16) && aligned(y, 16) && aligned(s, 16) &&
-                   (gate == nullptr || (aligned(gate, 16) && (gate_rows == 1 || ldgate % v == 0)));
+  const Access access = access_of(es, cols, {x, residual, weight, post_weight, gate, y, s}, {ldx, ldr, ldy, lds, gate != nullptr && gate_rows > 1 ? ldgate : 0});
   B200_DISPATCH_DTYPE(dtype, T, {
     ForwardArgs<T> a;
     a.x = static_cast<const T*>(x), a.residual = static_cast<const T*>(residual), a.weight = static_cast<const T*>(weight);
@@ -213,7 +220,7 @@ extern "C" int b200_gated_add_rms_norm(const void* x, const void* residual, cons
     a.inv_cols = 1.f / static_cast<float>(cols), a.eps = static_cast<float>(eps), a.offset = static_cast<float>(offset);
     a.scale = static_cast<float>(scale), a.residual_scale = static_cast<float>(residual_scale), a.act = activation;
     a.words = 0;
-    return run_forward<T>(a, cols, vec, static_cast<cudaStream_t>(stream));
+    return run_forward<T>(a, cols, access, static_cast<cudaStream_t>(stream));
   });
   return B200_OK;
 }

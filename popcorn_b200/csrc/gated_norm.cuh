@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 
 #include "activations.cuh"
 #include "common.cuh"
@@ -13,11 +14,13 @@ namespace {
 
 enum Activation { kIdentity = 0, kTanh = 1, kSigmoid = 2 };
 
-// One load: a 128-bit word of T, or one element where width, strides or pointers do not allow words.
-template <typename T, bool VEC>
+// One load: a 128-bit word of T, or where width, strides or pointers do not allow words, two neighbouring elements at once, or
+// where they do not allow that either, one element.
+enum Access { kWords = 0, kPairs = 1, kSingles = 2 };
+template <typename T, int ACCESS>
 struct Word;
 template <typename T>
-struct Word<T, true> {
+struct Word<T, kWords> {
   static constexpr int N = Num<T>::kVec;
   using Raw = uint4;
   static __device__ __forceinline__ Raw zero() { return make_uint4(0, 0, 0, 0); }
@@ -27,7 +30,19 @@ struct Word<T, true> {
   static __device__ __forceinline__ void store(T* p, const float (&f)[N]) { st_stream(p, Num<T>::pack(f)); }
 };
 template <typename T>
-struct Word<T, false> {
+struct Word<T, kPairs> {
+  static constexpr int N = 2;
+  struct alignas(2 * sizeof(T)) Raw {
+    T lo, hi;
+  };
+  static __device__ __forceinline__ Raw zero() { return {Num<T>::down(0.f), Num<T>::down(0.f)}; }
+  static __device__ __forceinline__ Raw load(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+  static __device__ __forceinline__ Raw load_shared_by_rows(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[2]) { f[0] = Num<T>::up(r.lo), f[1] = Num<T>::up(r.hi); }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[2]) { *reinterpret_cast<Raw*>(p) = {Num<T>::down(f[0]), Num<T>::down(f[1])}; }
+};
+template <typename T>
+struct Word<T, kSingles> {
   static constexpr int N = 1;
   using Raw = T;
   static __device__ __forceinline__ Raw zero() { return Num<T>::down(0.f); }
@@ -262,8 +277,12 @@ __device__ __forceinline__ uint32_t range_start(uint32_t rows, int walkers, int 
   return static_cast<uint32_t>(static_cast<uint64_t>(rows) * walker / walkers);
 }
 
-// What a thread loads at a time, as fp32 pairs (two elements per instruction): a 128-bit word, or two neighbouring elements
-// of which the second may lie behind the row.
+// What a thread of a walker loads at a time, as fp32 pairs (two elements per instruction): a 128-bit word, or two neighbouring
+// elements, together where all rows allow it (RowShape::pairs), else one after the other, the second perhaps behind the row.
+struct RowShape {
+  int cols;
+  bool pairs;
+};
 template <typename T, bool VEC>
 struct Pairs {
   static constexpr int P = Num<T>::kVec / 2, N = 2 * P;
@@ -273,9 +292,9 @@ struct Pairs {
 #pragma unroll
     for (int j = 0; j < P; ++j) out[j] = pack_f2(f[2 * j], f[2 * j + 1]);
   }
-  static __device__ __forceinline__ void load(const RowView& v, int w, int, Float2x (&out)[P]) { unpack(ld_shared(v.memory + w * 16), out); }
-  static __device__ __forceinline__ void load_shared_by_rows(const T* row, int w, int, Float2x (&out)[P]) { unpack(ld_kept(row + w * N), out); }
-  static __device__ __forceinline__ void store(T* row, int w, int, const Float2x (&v)[P]) {
+  static __device__ __forceinline__ void load(const RowView& v, int w, RowShape, Float2x (&out)[P]) { unpack(ld_shared(v.memory + w * 16), out); }
+  static __device__ __forceinline__ void load_shared_by_rows(const T* row, int w, RowShape, Float2x (&out)[P]) { unpack(ld_kept(row + w * N), out); }
+  static __device__ __forceinline__ void store(T* row, int w, RowShape, const Float2x (&v)[P]) {
     float f[N];
 #pragma unroll
     for (int j = 0; j < P; ++j) unpack_f2(v[j], f[2 * j], f[2 * j + 1]);
@@ -298,17 +317,42 @@ struct Pairs<T, false> {
       return Num<T>::up(*reinterpret_cast<const T*>(&bits));
     }
   }
-  static __device__ __forceinline__ void load(const RowView& v, int w, int cols, Float2x (&out)[1]) {
-    out[0] = pack_f2(element(v, 2 * w), 2 * w + 1 < cols ? element(v, 2 * w + 1) : 0.f);
+  using Two = Word<T, kPairs>;
+  static __device__ __forceinline__ Float2x as_pair(const typename Two::Raw& raw) {
+    float f[2];
+    Two::unpack(raw, f);
+    return pack_f2(f[0], f[1]);
   }
-  static __device__ __forceinline__ void load_shared_by_rows(const T* row, int w, int cols, Float2x (&out)[1]) {
-    out[0] = pack_f2(Num<T>::up(row[2 * w]), 2 * w + 1 < cols ? Num<T>::up(row[2 * w + 1]) : 0.f);
+  static __device__ __forceinline__ void load(const RowView& v, int w, RowShape shape, Float2x (&out)[1]) {
+    if (shape.pairs) {
+      const uint32_t byte = static_cast<uint32_t>(w) * 2 * static_cast<uint32_t>(sizeof(T));
+      if (byte < v.lo || byte >= v.hi) {
+        out[0] = as_pair(Two::load(static_cast<const T*>(v.row) + 2 * w));
+      } else if constexpr (sizeof(T) == 4) {
+        float lo, hi;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(lo), "=f"(hi) : "r"(v.memory + byte) : "memory");
+        out[0] = pack_f2(lo, hi);
+      } else {
+        uint32_t bits;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bits) : "r"(v.memory + byte) : "memory");
+        out[0] = as_pair(*reinterpret_cast<const typename Two::Raw*>(&bits));
+      }
+      return;
+    }
+    out[0] = pack_f2(element(v, 2 * w), 2 * w + 1 < shape.cols ? element(v, 2 * w + 1) : 0.f);
   }
-  static __device__ __forceinline__ void store(T* row, int w, int cols, const Float2x (&v)[1]) {
-    float lo, hi;
-    unpack_f2(v[0], lo, hi);
-    row[2 * w] = Num<T>::down(lo);
-    if (2 * w + 1 < cols) row[2 * w + 1] = Num<T>::down(hi);
+  static __device__ __forceinline__ void load_shared_by_rows(const T* row, int w, RowShape shape, Float2x (&out)[1]) {
+    out[0] = pack_f2(Num<T>::up(row[2 * w]), 2 * w + 1 < shape.cols ? Num<T>::up(row[2 * w + 1]) : 0.f);
+  }
+  static __device__ __forceinline__ void store(T* row, int w, RowShape shape, const Float2x (&v)[1]) {
+    float f[2];
+    unpack_f2(v[0], f[0], f[1]);
+    if (shape.pairs) {
+      Two::store(row + 2 * w, f);
+      return;
+    }
+    row[2 * w] = Num<T>::down(f[0]);
+    if (2 * w + 1 < shape.cols) row[2 * w + 1] = Num<T>::down(f[1]);
   }
 };
 __device__ __forceinline__ Float2x both(float v) { return pack_f2(v, v); }
@@ -372,6 +416,18 @@ int allow_smem(const char* name) {
     return fail(B200_ERR_LAUNCH, "%s: %s", name, cudaGetErrorString(cudaGetLastError()));
   done.fetch_or(bit, std::memory_order_release);
   return B200_OK;
+}
+
+// The widest access that the width, the strides and the pointers of all operands (NULL: none) allow.
+Access access_of(size_t element, int64_t cols, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> strides) {
+  for (const Access access : {kWords, kPairs}) {
+    const int64_t elements = access == kWords ? 16 / static_cast<int64_t>(element) : 2;
+    bool fits = cols % elements == 0;
+    for (const void* p : pointers) fits = fits && aligned(p, elements * element);
+    for (const int64_t ld : strides) fits = fits && ld % elements == 0;
+    if (fits) return access;
+  }
+  return kSingles;
 }
 
 // Sizes and enums that both directions check alike.

@@ -30,6 +30,7 @@ struct BackwardArgs {
   float *weight_lines, *branch_lines;
   uint32_t rows, period;
   int columns, walkers;
+  bool pairs;
   int64_t ldgy, ldgs, ldx, ldr, ldgate, ldo;
   float inv_cols, offset, scale, residual_scale;
   int act;
@@ -41,6 +42,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
   using PW = Pairs<T, VEC>;
   constexpr int N = PW::N, P = PW::P, ITEMS = kColumns / N;
   const int cols = a.columns, words = (cols + N - 1) / N;
+  const RowShape shape = {cols, a.pairs};
   extern __shared__ __align__(128) unsigned char memory[];
   __shared__ uint64_t barriers[kMaxSlots];
   __shared__ int flag;
@@ -65,7 +67,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
 #pragma unroll
     for (int j = 0; j < P; ++j) weight[i][j] = sum_w[i][j] = sum_k[i][j] = both(0.f);
     if (ok[i]) {
-      PW::load_shared_by_rows(a.weight, w, cols, weight[i]);
+      PW::load_shared_by_rows(a.weight, w, shape, weight[i]);
 #pragma unroll
       for (int j = 0; j < P; ++j) weight[i][j] = add_f2(weight[i][j], offset2);
     }
@@ -80,12 +82,12 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       if (!ok[i]) continue;
       Float2x v[P];
       if (a.post != nullptr) {
-        PW::load_shared_by_rows(a.post, w, cols, v);
+        PW::load_shared_by_rows(a.post, w, shape, v);
 #pragma unroll
         for (int j = 0; j < P; ++j) factor[i][j] = mul_f2(factor[i][j], add_f2(v[j], offset2));
       }
       if (!ROW_GATE && a.gate != nullptr) {
-        PW::load_shared_by_rows(a.gate + static_cast<int64_t>(gate_row) * a.ldgate, w, cols, v);
+        PW::load_shared_by_rows(a.gate + static_cast<int64_t>(gate_row) * a.ldgate, w, shape, v);
 #pragma unroll
         for (int j = 0; j < P; ++j) factor[i][j] = mul_f2(factor[i][j], activate2<T>(v[j], a.act));
       }
@@ -139,13 +141,13 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       if (!ok[i]) continue;
       const int w = lane_in_row + i * TPR;
       Float2x x[P], res[P], gy[P], gs[P];
-      PW::load(xv, w, cols, x);
-      PW::load(rv, w, cols, res);
-      PW::load(gyv, w, cols, gy);
-      if constexpr (ROW_GATE) PW::load(gv, w, cols, value[i]);
+      PW::load(xv, w, shape, x);
+      PW::load(rv, w, shape, res);
+      PW::load(gyv, w, shape, gy);
+      if constexpr (ROW_GATE) PW::load(gv, w, shape, value[i]);
 #pragma unroll
       for (int j = 0; j < P; ++j) gs[j] = both(0.f);
-      if (has_gs) PW::load(gsv, w, cols, gs);
+      if (has_gs) PW::load(gsv, w, shape, gs);
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         Float2x f = factor[i][j];
@@ -178,12 +180,12 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       const int w = lane_in_row + i * TPR;
       const int64_t at = row * a.ldo;
       Float2x x[P], res[P], gy[P], gs[P], g[P];
-      PW::load(xv, w, cols, x);
-      PW::load(rv, w, cols, res);
-      PW::load(gyv, w, cols, gy);
+      PW::load(xv, w, shape, x);
+      PW::load(rv, w, shape, res);
+      PW::load(gyv, w, shape, gy);
 #pragma unroll
       for (int j = 0; j < P; ++j) gs[j] = both(0.f);
-      if (has_gs) PW::load(gsv, w, cols, gs);
+      if (has_gs) PW::load(gsv, w, shape, gs);
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         Float2x f = factor[i][j];
@@ -204,9 +206,9 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
         x[j] = fma_f2(f, mul_f2(r12, ds), mul_f2(minus_c1, xr));
         res[j] = mul_f2(residual_scale2, ds);
       }
-      PW::store(a.dx + at, w, cols, x);
-      PW::store(a.dresidual + at, w, cols, res);
-      if constexpr (ROW_GATE) PW::store(a.dgate + at, w, cols, g);
+      PW::store(a.dx + at, w, shape, x);
+      PW::store(a.dresidual + at, w, shape, res);
+      if constexpr (ROW_GATE) PW::store(a.dgate + at, w, shape, g);
     }
     if (TPR == 32 || tight) {
       __syncthreads();
@@ -404,7 +406,6 @@ int run_backward(BackwardArgs<T> a, ColumnArgs<T> c, int64_t cols, const Backwar
     launch(gated_backward_wide_kernel<T>, static_cast<unsigned>(a.walkers), kBackwardThreads, 0, st, a, cols, row_gate);
     rc = after_launch("gated_backward_wide_kernel");
   } else {
-    vec = vec && cols % Num<T>::kVec == 0;
     rc = vec ? run_walk_back<T, true>(a, p.w, row_gate, st) : run_walk_back<T, false>(a, p.w, row_gate, st);
   }
   if (rc) return rc;
@@ -454,11 +455,8 @@ extern "C" int b200_gated_add_rms_norm_backward(const void* grad_y, const void* 
     return fail(B200_ERR_NULL_POINTER, "%s: post_weight and grad_post_weight, gate and grad_gate go together", __func__);
   const size_t es = dtype_size(dtype);
   const void* all[] = {grad_y, grad_s, x, residual, weight, post_weight, gate, grad_x, grad_residual, grad_weight, grad_post_weight, grad_gate};
-  bool words = true;
-  for (const void* p : all) {
+  for (const void* p : all)
     if (!aligned(p, es)) return fail(B200_ERR_ALIGNMENT, "%s: pointer not aligned to the element size", __func__);
-    words = words && aligned(p, 16);
-  }
   if (!aligned(stats, 8)) return fail(B200_ERR_ALIGNMENT, "%s: stats must be 8-byte aligned", __func__);
   if (int rc = check_device()) return rc;
   if (rows == 0) {
@@ -468,9 +466,8 @@ extern "C" int b200_gated_add_rms_norm_backward(const void* grad_y, const void* 
       return fail(B200_ERR_LAUNCH, "%s: %s", __func__, cudaGetErrorString(cudaGetLastError()));
     return B200_OK;
   }
-  const int64_t v = 16 / static_cast<int64_t>(es);
-  words = words && ldgy % v == 0 && (grad_s == nullptr || ldgs % v == 0) && ldx % v == 0 && ldr % v == 0 &&
-          (gate == nullptr || gate_rows <= 1 || ldgate % v == 0);
+  const Access access = access_of(es, cols, {grad_y, grad_s, x, residual, weight, post_weight, gate, grad_x, grad_residual, grad_gate},
+                                  {ldgy, grad_s == nullptr ? 0 : ldgs, ldx, ldr, gate != nullptr && gate_rows > 1 ? ldgate : 0});
   const BackwardPlan p = plan_backward(rows, cols, gate == nullptr ? 0 : gate_rows, es);
   const size_t need = static_cast<size_t>(p.weight_lines + p.branch_lines) * static_cast<size_t>(cols) * sizeof(float);
   if (scratch_bytes < need || !aligned(scratch, 16))
@@ -486,7 +483,7 @@ extern "C" int b200_gated_add_rms_norm_backward(const void* grad_y, const void* 
     a.weight_lines = static_cast<float*>(scratch);
     a.branch_lines = post_weight == nullptr && !shared_gate ? nullptr : a.weight_lines + p.weight_lines * cols;
     a.rows = static_cast<uint32_t>(rows), a.period = shared_gate ? static_cast<uint32_t>(rows / gate_rows) : 1;
-    a.columns = static_cast<int>(cols), a.walkers = p.w.walkers;
+    a.columns = static_cast<int>(cols), a.walkers = p.w.walkers, a.pairs = access == kPairs;
     a.ldgy = ldgy, a.ldgs = ldgs, a.ldx = ldx, a.ldr = ldr, a.ldgate = ldgate, a.ldo = cols;
     a.inv_cols = 1.f / static_cast<float>(cols), a.offset = static_cast<float>(offset), a.scale = static_cast<float>(scale);
     a.residual_scale = static_cast<float>(residual_scale), a.act = activation;
@@ -496,7 +493,7 @@ extern "C" int b200_gated_add_rms_norm_backward(const void* grad_y, const void* 
     c.cols = cols, c.ldgate = ldgate, c.rows = a.rows, c.period = a.period;
     c.walkers = p.w.walkers, c.gate_rows = shared_gate ? static_cast<int>(gate_rows) : 0;
     c.offset = a.offset, c.scale = a.scale, c.line_scale = gate == nullptr ? a.scale : 1.f, c.act = activation;
-    return run_backward<T>(a, c, cols, p, words, row_gate, static_cast<cudaStream_t>(stream));
+    return run_backward<T>(a, c, cols, p, access == kWords, row_gate, static_cast<cudaStream_t>(stream));
   });
   return B200_OK;
 }
