@@ -164,20 +164,22 @@ int run_forward(ForwardArgs<T> a, int64_t cols, Access access, cudaStream_t st) 
     return launch_forward<T, kWords, 1024, 4>(a, st);
   }
   // two elements at a time keep half as many instructions busy for the same bytes ([4095, 2050] fp32 with a gate per row:
-  // PAIRS us, one element at a time 57)
+  // 47 us, one element at a time 57; [8192, 2050] bf16 64 and 86)
   if (access != kSingles && cols <= 16384) {
     a.words = static_cast<int>(cols / 2);
-    if (a.words <= 128) return launch_forward<T, kPairs, 32, 4>(a, st);
-    if (a.words <= 1024) return launch_forward<T, kPairs, 256, 4>(a, st);
-    if (a.words <= 2048) return launch_forward<T, kPairs, 512, 4>(a, st);
-    if (a.words <= 4096) return launch_forward<T, kPairs, 512, 8>(a, st);
-    return launch_forward<T, kPairs, 1024, 8>(a, st);
+    if (a.words <= 256) return launch_forward<T, kPairs, 32, 8>(a, st);
+    if (a.words <= 1024) return launch_forward<T, kPairs, 128, 8>(a, st);
+    if (a.words <= 1536) return launch_forward<T, kPairs, 128, 12>(a, st);
+    if (a.words <= 2048) return launch_forward<T, kPairs, 128, 16>(a, st);
+    if (a.words <= 4096) return launch_forward<T, kPairs, 256, 16>(a, st);
+    return launch_forward<T, kPairs, 512, 16>(a, st);
   }
   if (cols <= 16384) {
     a.words = static_cast<int>(cols);
     if (cols <= 256) return launch_forward<T, kSingles, 32, 8>(a, st);
-    if (cols <= 2048) return launch_forward<T, kSingles, 256, 8>(a, st);
-    if (cols <= 4096) return launch_forward<T, kSingles, 512, 8>(a, st);
+    if (cols <= 1024) return launch_forward<T, kSingles, 128, 8>(a, st);
+    if (cols <= 2048) return launch_forward<T, kSingles, 128, 16>(a, st);
+    if (cols <= 4096) return launch_forward<T, kSingles, 256, 16>(a, st);
     if (cols <= 8192) return launch_forward<T, kSingles, 512, 16>(a, st);
     return launch_forward<T, kSingles, 1024, 16>(a, st);
   }

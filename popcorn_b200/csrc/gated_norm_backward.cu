@@ -114,6 +114,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
   }
   load_factor(gate_row);
   const Float2x residual_scale2 = both(a.residual_scale), scale2 = both(a.scale);
+  const RowAct row_act = make_row_act(a.act);
   const bool tight = slots < 2 * ring.count;  // the next row's copies need slots of this one: a barrier of their own at its end
   float2 stat = first < last ? a.stats[first] : make_float2(0.f, 0.f);  // of the next row: its latency is that of a row
   int parity = 0;
@@ -144,17 +145,17 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       PW::load(xv, w, shape, x);
       PW::load(rv, w, shape, res);
       PW::load(gyv, w, shape, gy);
-      if constexpr (ROW_GATE) PW::load(gv, w, shape, value[i]);
+      if constexpr (ROW_GATE) {
+        PW::load(gv, w, shape, value[i]);
+        activate_row(value[i], row_act);
+      }
 #pragma unroll
       for (int j = 0; j < P; ++j) gs[j] = both(0.f);
       if (has_gs) PW::load(gsv, w, shape, gs);
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         Float2x f = factor[i][j];
-        if constexpr (ROW_GATE) {
-          value[i][j] = activate2<T>(value[i][j], a.act);
-          f = mul_f2(f, value[i][j]);
-        }
+        if constexpr (ROW_GATE) f = mul_f2(f, value[i][j]);
         const Float2x u = mul_f2(f, mul_f2(r12, x[j]));
         const Float2x s = fma_f2(residual_scale2, res[j], u);
         const Float2x gw = mul_f2(gy[j], weight[i][j]);
@@ -199,7 +200,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
           sum_k[i][j] = fma_f2(mul_f2(scale2, value[i][j]), k, sum_k[i][j]);
           float lo, hi;
           unpack_f2(value[i][j], lo, hi);
-          g[j] = mul_f2(mul_f2(factor[i][j], pack_f2(activation_slope(lo, a.act), activation_slope(hi, a.act))), k);
+          g[j] = mul_f2(mul_f2(factor[i][j], pack_f2(row_slope(lo, row_act), row_slope(hi, row_act))), k);
         } else {
           sum_k[i][j] = fma_f2(ds, xr, sum_k[i][j]);
         }
