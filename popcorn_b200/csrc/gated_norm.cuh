@@ -134,7 +134,6 @@ __device__ __forceinline__ void row_sums(float (&v)[4], float (*slot)[16]) {
 // A bulk copy moves multiples of 16 bytes between 16-byte boundaries: of a row that starts or ends elsewhere the ring
 // holds what lies between, [lo, hi) in bytes from the row's start, and the few elements around it are loaded directly.
 constexpr int kMaxSlots = 16;
-constexpr int kMaxArrays = 5;
 
 __device__ __forceinline__ uint4 ld_shared(uint32_t at) {
   uint4 v;
@@ -430,7 +429,7 @@ WalkPlan plan_walk(int64_t rows, int64_t cols, size_t element) {
   const int per_sm = kMaxWalk / p.tpr;
   p.walkers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, static_cast<int64_t>(sm_count()) * per_sm)));
   p.slot_bytes = static_cast<uint32_t>(std::max<int64_t>(1, ceil_div(cols * static_cast<int64_t>(element), 16)) * 16);
-  p.slots = static_cast<int>(std::min<size_t>(kMaxSlots, kRingBytes / per_sm / p.slot_bytes));  // at least 6: a row's arrays fit
+  p.slots = static_cast<int>(std::min<size_t>(kMaxSlots, kRingBytes / per_sm / p.slot_bytes));  // at least 6: a row's arrays, five at most, fit
   return p;
 }
 

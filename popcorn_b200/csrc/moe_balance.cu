@@ -11,7 +11,7 @@
 // leaves one line of sums, a second small kernel adds the lines up in a fixed order in fp64 (a cluster per group, each CTA
 // some of the experts).  Backward: the logits read again, the gradient written; row maximum and sum come from the forward
 // pass (8 bytes a token).  A lane has eight loads in flight, of one token or of several: with two, [131072, 256] fp32 took
-// 91 us forward instead of 35.
+// 91 us forward instead of 36.
 #include <algorithm>
 #include <type_traits>
 
