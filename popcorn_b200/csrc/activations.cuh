@@ -28,6 +28,13 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// a within [-88, 88]; a NaN stays one (fminf and fmaxf return their other operand)
+__device__ __forceinline__ float clamp_exponent(float a) {
+  float c;
+  asm("max.NaN.f32 %0, %1, 0fC2B00000;" : "=f"(c) : "f"(a));  // -88
+  asm("min.NaN.f32 %0, %1, 0f42B00000;" : "=f"(c) : "f"(c));  // 88
+  return c;
+}
 template <int MATH>
 __device__ __forceinline__ float exp_neg(float a) {
   if constexpr (MATH == 0) {
@@ -36,9 +43,8 @@ __device__ __forceinline__ float exp_neg(float a) {
     constexpr float kNegLog2e = -1.4426950216293335f;       // fp32(-log2(e))
     constexpr float kNegLog2eLo = -1.9259629911266175e-8f;  // -log2(e) - fp32(-log2(e))
     // |a| <= 88 keeps every intermediate finite (exp(88) < 2^127); beyond that the quotient
-    // below is 0 or a itself whatever the exponential is.  A NaN a becomes -88 here and is
-    // restored by the multiplication with a in silu_f32.
-    const float ac = fminf(fmaxf(a, -88.0f), 88.0f);
+    // below is 0 or a itself whatever the exponential is.
+    const float ac = clamp_exponent(a);
     const float t = __fmul_rn(ac, kNegLog2e);
     float lo = __fmaf_rn(ac, kNegLog2e, -t);  // what the rounding of t dropped
     lo = __fmaf_rn(ac, kNegLog2eLo, lo);

@@ -52,7 +52,7 @@ struct Word<T, kSingles> {
   static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { *p = Num<T>::down(f[0]); }
 };
 
-// tanh below 1/4: the next term of its series is below 1e-8 of it
+// tanh below 1/4: the next term of its series is below 1e-8 of it (a NaN is not below 1/4 and is kept by the sigmoid)
 __device__ __forceinline__ float tanh_series(float g) {
   const float q = g * g;
   return g * fmaf(q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);

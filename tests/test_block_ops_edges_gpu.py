@@ -1,0 +1,56 @@
+"""Calls at the edges of the operators around the layers: gates and logits that are no ordinary numbers, calls from several threads,
+derivatives that the kernels do not have."""
+
+import pytest
+import torch
+
+from popcorn_b200 import ops
+from tests.test_block_ops_gpu import BF16, DEV, F16, F32, check_norm, near, norm_inputs, norm_reference, normal
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+GATE_FORMS = [(hidden, dtype, activation, gate) for hidden, dtype in ((256, BF16), (256, F16), (256, F32), (130, BF16), (129, F16), (130, F32), (4096, BF16), (16390, F16), (16390, F32))
+              for activation in ("tanh", "sigmoid") for gate in ("channel", "first", "row")]
+
+
+@pytest.mark.parametrize("hidden,dtype,activation,gate", GATE_FORMS)
+def test_norm_gate_of_infinities_is_open_or_shut(hidden, dtype, activation, gate):
+    """tanh is 1 and -1 there, the sigmoid 1 and 0, both slopes 0: everything stays finite."""
+    inputs = norm_inputs(hidden, (3, 5), hidden, dtype, True, gate)
+    rows = inputs[4].view(-1, hidden)
+    rows[-1, 3], rows[-1, 8] = INF, -INF
+    gy, gs = normal(1, 3, 5, hidden, dtype=dtype), normal(2, 3, 5, hidden, dtype=dtype)
+    got = check_norm(*inputs, activation, gy=gy, gs=gs)
+    shut = got["gate"].view(-1, hidden)[-1]
+    assert shut[3] == 0 and shut[8] == 0
+
+
+@pytest.mark.parametrize("hidden,dtype,activation,gate", GATE_FORMS)
+def test_norm_gate_that_is_nan_shows(hidden, dtype, activation, gate):
+    """Where the definition gives NaN the outputs and gradients do, and nowhere else."""
+    inputs = norm_inputs(hidden, (3, 5), hidden, dtype, True, gate)
+    inputs[4].view(-1, hidden)[-1, 5] = NAN
+    gy, gs = normal(3, 3, 5, hidden, dtype=dtype), normal(4, 3, 5, hidden, dtype=dtype)
+    y, s, stats = ops.gated_add_rms_norm_forward(*inputs, activation)
+    grads = ops.gated_add_rms_norm_backward(gy, gs, *inputs, stats, activation)
+    want = norm_reference(*inputs, activation, 1.0, 1.0, 1e-6, 0.0, gy, gs)
+    assert want["s"][0].isnan().any() and not want["s"][0].isnan().all()
+    for name, got in zip(("y", "s", "x", "residual", "weight", "post", "gate"), (y, s, *grads)):
+        value, magnitude = want[name]
+        lost = value.isnan()
+        assert torch.equal(got.isnan(), lost), name
+        near(torch.where(lost, 0.0, got).to(dtype), torch.where(lost, 0.0, value), torch.where(lost, 0.0, magnitude), roundings=96 + 15, what=name)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_rms_norm_gated_by_a_sigmoid_of_nan(dtype):
+    """The sigmoid is the one of the gated norm."""
+    x, g, weight = normal(1, 4, 64, dtype=dtype), normal(2, 4, 64, dtype=dtype), torch.ones(64, dtype=dtype, device=DEV)
+    g[2, 9] = NAN
+    for activation in ("sigmoid", "swish"):
+        got = ops.rms_norm_gated(x, g, weight, activation=activation).isnan()
+        assert got[2, 9] and int(got.sum()) == 1
+    for backward in (ops.sigmoid_gate_backward, ops.swiglu_backward):
+        da, db = backward(x, g, x)
+        assert da[2, 9].isnan() and db[2, 9].isnan() and int(da.isnan().sum()) == int(db.isnan().sum()) == 1
