@@ -413,7 +413,7 @@ int b200_moe_balance_loss_backward(const void* logits, const uint8_t* mask, cons
 /*
  * out[t, :] = round_T(scale * weight[ids[t], :]).  ids: int32, or int64 if ids_64 != 0.  An id outside [0, vocab) gives a
  * row of zeros (a shard of a table is passed with the ids shifted by its first row).  weight: [vocab, cols] with row stride
- * ldw; cols <= 65535 * 128, tokens <= 2^30, vocab < 2^31.  The row gather of b200_moe_gather with the ids of a batch.
+ * ldw; cols <= 65535 * 128, tokens <= 2^30, vocab <= 2^31 - 2^16.  The row gather of b200_moe_gather with the ids of a batch.
  */
 int b200_embedding(const void* ids, const void* weight, void* out, int64_t tokens, int64_t vocab, int64_t cols, int64_t ldw,
                    int64_t ldo, int ids_64, int dtype, double scale, void* stream);

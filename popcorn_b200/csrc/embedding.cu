@@ -470,10 +470,13 @@ size_t scratch_layout(int64_t tokens, int64_t vocab, int64_t cols, char* base, S
   return at;
 }
 
+// The join kernel counts rows in 32 bits, and each of its 2 * 8 * (SMs) filling warps goes eight rows past the last one to find
+// that it is done: room for that below 2^31, for up to 512 SMs.
+constexpr int64_t kMaxVocab = (1LL << 31) - (1LL << 16);
 int check_sizes(const char* fn, int64_t tokens, int64_t vocab, int64_t cols, int dtype) {
   if (!dtype_ok(dtype)) return fail(B200_ERR_DTYPE, "%s: unsupported dtype %d", fn, dtype);
   if (tokens < 0 || vocab < 0 || cols < 0) return fail(B200_ERR_SHAPE, "%s: negative size", fn);
-  if (tokens > (1LL << 30) || vocab > 0x7fffffffLL) return fail(B200_ERR_SHAPE, "%s: tokens=%lld exceeds 2^30 or vocab=%lld 2^31-1", fn, (long long)tokens, (long long)vocab);
+  if (tokens > (1LL << 30) || vocab > kMaxVocab) return fail(B200_ERR_SHAPE, "%s: tokens=%lld exceeds 2^30 or vocab=%lld 2^31-2^16", fn, (long long)tokens, (long long)vocab);
   if (cols > 65535LL * 128) return fail(B200_ERR_SHAPE, "%s: cols=%lld exceeds %lld", fn, (long long)cols, 65535LL * 128);
   return B200_OK;
 }
