@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/popcorn_b200.h"
 
 namespace b200 {
@@ -65,6 +67,22 @@ inline void launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem
   config.attrs = attr;
   config.numAttrs = pdl_enabled() ? 1 : 0;
   (void)cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+}
+
+// Opt in to more than 48 KB of shared memory, once per kernel and device.  BYTES: the most that any launch of the kernel takes.
+// The setting belongs to the kernel and not to the launch: set to each launch's own size, another thread's smaller one could come
+// between the two, and the launch would fail.
+template <auto kernel, int BYTES>
+int allow_smem(const char* name) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return fail(B200_ERR_DEVICE, "%s: no current device", name);
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return B200_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) != cudaSuccess)
+    return fail(B200_ERR_LAUNCH, "%s: %s", name, cudaGetErrorString(cudaGetLastError()));
+  done.fetch_or(bit, std::memory_order_release);
+  return B200_OK;
 }
 
 #define B200_REQUIRE_PTR(p)                                                        \

@@ -490,9 +490,8 @@ int run_backward(const void* grad_out, const void* ids, void* grad_weight, int64
   const bool vec = cols % V == 0 && ldg % V == 0 && aligned(g, 16) && aligned(out, 16);
   const int range = static_cast<int>(ceil_div(vocab, order_ctas(vocab)));
   const size_t smem = static_cast<size_t>(range) * kListWarps * sizeof(int);
-  auto order = embedding_order_kernel<T, I>;
-  if (cudaFuncSetAttribute(order, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
-    return fail(B200_ERR_LAUNCH, "embedding_order_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+  constexpr auto order = embedding_order_kernel<T, I>;
+  if (int rc = allow_smem<order, kMaxRange * kListWarps * static_cast<int>(sizeof(int))>("embedding_order_kernel")) return rc;
   const int pad = padding >= 0 && padding < vocab ? static_cast<int>(padding) : -1;
   launch(order, static_cast<unsigned>(ceil_div(vocab, range)), kOrderThreads, smem, st, static_cast<const I*>(ids), static_cast<int>(tokens), vocab, pad,
          range, s.token, s.id, s.count, s.hit, s.resume, out, cols);

@@ -2,7 +2,6 @@
 #pragma once
 
 #include <algorithm>
-#include <atomic>
 #include <initializer_list>
 
 #include "activations.cuh"
@@ -431,20 +430,6 @@ WalkPlan plan_walk(int64_t rows, int64_t cols, size_t element) {
   p.slot_bytes = static_cast<uint32_t>(std::max<int64_t>(1, ceil_div(cols * static_cast<int64_t>(element), 16)) * 16);
   p.slots = static_cast<int>(std::min<size_t>(kMaxSlots, kRingBytes / per_sm / p.slot_bytes));  // at least 6: a row's arrays, five at most, fit
   return p;
-}
-
-// Opt in to more than 48 KB of shared memory, once per kernel and device.
-template <auto kernel>
-int allow_smem(const char* name) {
-  static std::atomic<uint64_t> done{0};
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return fail(B200_ERR_DEVICE, "%s: no current device", name);
-  const uint64_t bit = device < 64 ? 1ull << device : 0;
-  if (done.load(std::memory_order_acquire) & bit) return B200_OK;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes) != cudaSuccess)
-    return fail(B200_ERR_LAUNCH, "%s: %s", name, cudaGetErrorString(cudaGetLastError()));
-  done.fetch_or(bit, std::memory_order_release);
-  return B200_OK;
 }
 
 // The widest access that the width, the strides and the pointers of all operands (NULL: none) allow.

@@ -382,7 +382,7 @@ BackwardPlan plan_backward(int64_t rows, int64_t cols, int64_t gate_rows, size_t
 template <typename T, bool VEC, int TPR, bool ROW_GATE>
 int launch_backward(const BackwardArgs<T>& a, const WalkPlan& p, cudaStream_t st) {
   constexpr auto kernel = gated_backward_kernel<T, VEC, TPR, ROW_GATE>;
-  if (int rc = allow_smem<kernel>("gated_backward_kernel")) return rc;
+  if (int rc = allow_smem<kernel, kRingBytes>("gated_backward_kernel")) return rc;
   launch(kernel, static_cast<unsigned>(p.walkers), TPR, static_cast<size_t>(p.slots) * p.slot_bytes, st, a, p.slots, p.slot_bytes);
   return after_launch("gated_backward_kernel");
 }

@@ -1,10 +1,13 @@
 """Calls at the edges of the operators around the layers: gates and logits that are no ordinary numbers, calls from several threads,
 derivatives that the kernels do not have."""
 
+import threading
+import time
+
 import pytest
 import torch
 
-from popcorn_b200 import ops
+from popcorn_b200 import _lib, ops
 from tests.test_block_ops_gpu import BF16, DEV, F16, F32, check_norm, near, norm_inputs, norm_reference, normal
 
 pytestmark = pytest.mark.gpu
@@ -54,3 +57,38 @@ def test_rms_norm_gated_by_a_sigmoid_of_nan(dtype):
     for backward in (ops.sigmoid_gate_backward, ops.swiglu_backward):
         da, db = backward(x, g, x)
         assert da[2, 9].isnan() and db[2, 9].isnan() and int(da.isnan().sum()) == int(db.isnan().sum()) == 1
+
+
+def calls_from_threads(vocabs, seconds):
+    """Embedding gradients of tables of these sizes, each from a thread and on a stream of its own; the errors that they met."""
+    errors, stop = [], threading.Event()
+
+    def calls(vocab):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            ids, grad, out = torch.arange(16, device=DEV), torch.ones(16, 8, device=DEV), torch.empty(vocab, 8, device=DEV)
+            scratch = torch.empty(ops._scratch_bytes(0, "b200_embedding_backward_scratch_bytes", 16, vocab, 8), dtype=torch.uint8, device=DEV)
+        while not stop.is_set():
+            for _ in range(20):
+                try:
+                    _lib.call("b200_embedding_backward", grad.data_ptr(), ids.data_ptr(), out.data_ptr(), 16, vocab, 8, 8, -1, 1, _lib.F32, 1.0, scratch.data_ptr(),
+                              scratch.numel(), stream.cuda_stream)
+                except _lib.B200Error as error:
+                    errors.append(str(error))
+            stream.synchronize()
+        if not (bool((out[:16] == 1).all()) and not out[16:].any()):
+            errors.append(f"wrong gradient of {vocab} rows")
+
+    threads = [threading.Thread(target=calls, args=(vocab,)) for vocab in vocabs]
+    for thread in threads:
+        thread.start()
+    time.sleep(seconds)
+    stop.set()
+    for thread in threads:
+        thread.join()
+    return errors
+
+
+def test_embedding_gradients_of_small_and_large_tables_from_several_threads():
+    """The listing kernel's shared memory goes with the rows of the table: no call may narrow another's."""
+    assert not calls_from_threads((100, 100, 100, 100, 200000), 1.5)
