@@ -695,8 +695,9 @@ int run_bwd(const void* gy, const void* gs, const void* x, const void* w, void* 
     const size_t ring_bytes = use_ring ? stages * slot_bytes : 0;
 #define B200_BWD_KERNEL(ITEMS, BIAS, RING)                                                                               \
   do {                                                                                                                   \
-    auto kernel = rms_bwd_rows_kernel<T, ITEMS, ADD, BIAS, RING>;                                                        \
-    if (RING) (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ring_bytes)); \
+    constexpr auto kernel = rms_bwd_rows_kernel<T, ITEMS, ADD, BIAS, RING>;                                              \
+    if (RING)                                                                                                            \
+      if (int rc = allow_smem<kernel, static_cast<int>(kRingBytesPerCta)>("rms_bwd_rows_kernel")) return rc;             \
     launch(kernel, lines, 256, ring_bytes, st, tgy, tgs, tx, tw, tdx, part_w, part_b, rows, nvec, ldg, ldgs, ldx, lddx,    \
            cols_f, eps, offset, stages);                                                                                 \
   } while (0)

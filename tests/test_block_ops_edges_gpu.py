@@ -59,27 +59,25 @@ def test_rms_norm_gated_by_a_sigmoid_of_nan(dtype):
         assert da[2, 9].isnan() and db[2, 9].isnan() and int(da.isnan().sum()) == int(db.isnan().sum()) == 1
 
 
-def calls_from_threads(vocabs, seconds):
-    """Embedding gradients of tables of these sizes, each from a thread and on a stream of its own; the errors that they met."""
+def errors_from_threads(makers, seconds):
+    """Each maker's call, over and over, from a thread and on a stream of its own; what they raised."""
     errors, stop = [], threading.Event()
 
-    def calls(vocab):
+    def calls(make):
         stream = torch.cuda.Stream()
         with torch.cuda.stream(stream):
-            ids, grad, out = torch.arange(16, device=DEV), torch.ones(16, 8, device=DEV), torch.empty(vocab, 8, device=DEV)
-            scratch = torch.empty(ops._scratch_bytes(0, "b200_embedding_backward_scratch_bytes", 16, vocab, 8), dtype=torch.uint8, device=DEV)
+            call, is_right = make(stream)
         while not stop.is_set():
             for _ in range(20):
                 try:
-                    _lib.call("b200_embedding_backward", grad.data_ptr(), ids.data_ptr(), out.data_ptr(), 16, vocab, 8, 8, -1, 1, _lib.F32, 1.0, scratch.data_ptr(),
-                              scratch.numel(), stream.cuda_stream)
+                    call()
                 except _lib.B200Error as error:
                     errors.append(str(error))
             stream.synchronize()
-        if not (bool((out[:16] == 1).all()) and not out[16:].any()):
-            errors.append(f"wrong gradient of {vocab} rows")
+        if not is_right():
+            errors.append("wrong values")
 
-    threads = [threading.Thread(target=calls, args=(vocab,)) for vocab in vocabs]
+    threads = [threading.Thread(target=calls, args=(make,)) for make in makers]
     for thread in threads:
         thread.start()
     time.sleep(seconds)
@@ -91,4 +89,27 @@ def calls_from_threads(vocabs, seconds):
 
 def test_embedding_gradients_of_small_and_large_tables_from_several_threads():
     """The listing kernel's shared memory goes with the rows of the table: no call may narrow another's."""
-    assert not calls_from_threads((100, 100, 100, 100, 200000), 1.5)
+    def table_of(vocab):
+        def make(stream):
+            ids, grad, out = torch.arange(16, device=DEV), torch.ones(16, 8, device=DEV), torch.empty(vocab, 8, device=DEV)
+            scratch = torch.empty(ops._scratch_bytes(0, "b200_embedding_backward_scratch_bytes", 16, vocab, 8), dtype=torch.uint8, device=DEV)
+            return (lambda: _lib.call("b200_embedding_backward", grad.data_ptr(), ids.data_ptr(), out.data_ptr(), 16, vocab, 8, 8, -1, 1, _lib.F32, 1.0, scratch.data_ptr(),
+                                      scratch.numel(), stream.cuda_stream),
+                    lambda: bool((out[:16] == 1).all()) and not out[16:].any())
+        return make
+    assert not errors_from_threads([table_of(vocab) for vocab in (100, 100, 100, 100, 200000)], 1.5)
+
+
+def test_rms_norm_gradients_of_several_widths_from_several_threads():
+    """The ring of the plain norm's backward takes as many rows as fit: more shared memory at 4160 columns than at 6144."""
+    def width_of(hidden):
+        def make(stream):
+            x, grad, weight = normal(1, 4, hidden, dtype=BF16), normal(2, 4, hidden, dtype=BF16), torch.ones(hidden, dtype=BF16, device=DEV)
+            grad_x, grad_w = torch.empty_like(x), torch.empty_like(weight)
+            scratch = ops._norm_scratch(4, hidden, False, x.device)
+            want = ops.rms_norm_backward(grad, x, weight)
+            return (lambda: _lib.call("b200_rms_norm_backward", grad.data_ptr(), x.data_ptr(), weight.data_ptr(), grad_x.data_ptr(), grad_w.data_ptr(), None, 4, hidden,
+                                      hidden, hidden, hidden, _lib.BF16, 1e-6, scratch.data_ptr(), scratch.numel(), stream.cuda_stream),
+                    lambda: torch.equal(grad_x, want[0]) and torch.equal(grad_w, want[1]))
+        return make
+    assert not errors_from_threads([width_of(hidden) for hidden in (6144, 6144, 6144, 6144, 4160)], 1.5)
