@@ -128,8 +128,11 @@ __device__ __forceinline__ void row_sums(float (&v)[4], float (*slot)[16]) {
 // r * arrays + a, in slot (r * arrays + a) % slots, so any number of slots above `arrays` keeps copies in flight.  The
 // copies of a row complete one barrier, barrier r % rows_ahead.  A thread for each array issues them; a slot is filled
 // again once the walker is past a barrier behind its last read.
-// Every wait is bounded: when one runs out, the walker stops issuing, its threads fetch what they read of the remaining
-// rows with ordinary loads (the data is the same), and it waits, bounded again, for what is in flight before it leaves.
+// Every wait is bounded.  A thread whose wait runs out fetches what it reads of that row with ordinary loads (a copy that
+// lands beside them brings the same data) and leaves the row's number in `broken`.  Behind the row's next barrier all
+// threads see it and agree: nothing is issued any more, the copies in flight are waited for, bounded again, and the
+// remaining rows are fetched with ordinary loads, into slots that no copy can reach.  Should that second wait run out as
+// well, a late copy could: the remaining rows, if in words, give NaN.
 // A bulk copy moves multiples of 16 bytes between 16-byte boundaries: of a row that starts or ends elsewhere the ring
 // holds what lies between, [lo, hi) in bytes from the row's start, and the few elements around it are loaded directly.
 constexpr int kMaxSlots = 16;
@@ -153,7 +156,7 @@ struct RowView {
 template <typename T, bool VEC, int TPR>
 struct Ring {
   uint32_t full, memory;  // shared-memory addresses
-  uint32_t broken;  // shared-memory address of the walker's flag
+  uint32_t broken;  // shared-memory address of 0, or 1 + the row (from the walker's first) whose wait ran out; behind it: 1, the wait for the rest did too
   int count, slots, rows_ahead;
   uint32_t row_bytes, slot_bytes;
   // the issuing threads (the first `count` of the walker, one array each): their array and the next row of it
@@ -167,25 +170,21 @@ struct Ring {
 
   // memory: slots * slot_bytes of this walker; all threads of the CTA call this.  array(a, base, ld) names the rows of array a.
   template <typename Arrays>
-  __device__ __forceinline__ void start(uint64_t* barriers, unsigned char* mem, int* flag, int n, uint32_t bytes, uint32_t padded, uint32_t first, uint32_t last, int arrays, Arrays&& array) {
-    full = smem_addr(barriers), memory = smem_addr(mem), broken = smem_addr(flag);
+  __device__ __forceinline__ void start(uint64_t* barriers, unsigned char* mem, uint32_t (&flags)[2], int n, uint32_t bytes, uint32_t padded, uint32_t first, uint32_t last, int arrays,
+                                        Arrays&& array) {
+    full = smem_addr(barriers), memory = smem_addr(mem), broken = smem_addr(flags);
     count = arrays, slots = n, row_bytes = bytes, slot_bytes = padded, put_row = first_row = first, last_row = last;
     rows_ahead = (slots + count - 1) / count;  // a barrier is used again only after the row before was given free
     put_copy = put = threadIdx.x;
     put_bar = take = take_bar = 0, phase = 0;
     array(static_cast<int>(threadIdx.x), base, ld);
     if (threadIdx.x == 0) {
-      *flag = 0;
+      flags[0] = flags[1] = 0;
       for (int k = 0; k < rows_ahead; ++k) mbar_init(barriers + k, count);
       mbar_init_fence();
     }
     __syncthreads();
     if (threadIdx.x < count) issue(slots);
-  }
-  __device__ __forceinline__ bool is_broken() const {
-    uint32_t v;
-    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(broken) : "memory");
-    return v != 0;
   }
   // bytes of a row that the ring holds, from the row's start
   __device__ __forceinline__ void span(const T* row, uint32_t& lo, uint32_t& hi) const {
@@ -215,12 +214,29 @@ struct Ring {
       if (++put_bar == rows_ahead) put_bar = 0;
     }
   }
-  // the walker is past a barrier behind its last read of the first `rows` rows
-  __device__ __forceinline__ void release(uint32_t rows) {
-    if (threadIdx.x < count && !is_broken()) issue(static_cast<int64_t>(rows) * count + slots);
+  static __device__ __forceinline__ uint32_t read_flag(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
   }
-  static __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+  static __device__ __forceinline__ void write_flag(uint32_t at, uint32_t v) { asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+  // All threads, past a barrier behind the wait for row `row`, with `free` rows read for the last time: their slots go to the next rows.
+  __device__ __forceinline__ void release(uint32_t row, uint32_t free) {
+    if (threadIdx.x >= count) return;
+    const uint32_t at = read_flag(broken);  // a thread that is ahead may have left the next row's number: that counts behind its barrier
+    if (at == 0 || at > row + 1) issue(static_cast<int64_t>(free) * count + slots);
+  }
+  // Have all copies landed that were issued with `free` rows given free, those from row `row` on among them?  put: the next row of
+  // this thread's array, `rows` or above if it issues none.  A call: the registers of the loop around are not to make room for it.
+  static __device__ __noinline__ bool drain(uint32_t full, int count, int slots, int rows_ahead, uint32_t put, uint32_t rows, uint32_t row, uint32_t free) {
+    rows = static_cast<uint32_t>(min((static_cast<int64_t>(free) * count + slots + count - 1) / count, static_cast<int64_t>(rows)));  // of which a copy was issued
+    for (; put < rows; ++put) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full + put % rows_ahead * 8) : "memory");  // the last one's other arrays: without a copy
+    bool landed = true;
+    for (; row < rows; ++row) landed = wait_for(full + row % rows_ahead * 8, row / rows_ahead & 1u, kSpinLimit) && landed;
+    return landed;
+  }
+  static __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, uint32_t limit) {
+    for (uint32_t i = 0; i < limit; ++i) {
       uint32_t done;
       asm volatile(
           "{\n\t.reg .pred p;\n\t"
@@ -234,12 +250,17 @@ struct Ring {
     atomicAdd(&g_wait_timeouts, 1u);
     return false;
   }
-  // the next row in turn: has it landed?
-  __device__ __forceinline__ bool wait() {
-    bool landed = !is_broken();
-    if (landed && !wait_for(full + take_bar * 8, phase)) {
-      asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(broken), "r"(1) : "memory");
-      landed = false;
+  // the next row in turn, row `row` from the walker's first: has it landed?  late: rows are given free at their own end, else at the
+  // first barrier of the row behind them
+  __device__ __forceinline__ bool wait(uint32_t row, uint32_t probes, bool late) {
+    const uint32_t at = read_flag(broken);
+    bool landed = at == 0 || at > row;
+    if (landed) {
+      landed = wait_for(full + take_bar * 8, phase, probes);
+      if (!landed) write_flag(broken, row + 1);
+    } else if (at == row) {  // the row before was the broken one, and the last given free were those before it
+      const uint32_t rows = last_row - first_row;
+      if (!drain(full, count, slots, rows_ahead, threadIdx.x < count ? put_row - first_row : rows, rows, row - 1, late ? row - 1 : row < 2 ? 0 : row - 2)) write_flag(broken + 4, 1);
     }
     if (++take_bar == rows_ahead) {
       take_bar = 0;
@@ -247,6 +268,8 @@ struct Ring {
     }
     return landed;
   }
+  // a row that has not landed: may a late copy reach its words?
+  __device__ __forceinline__ bool unsound() const { return VEC && read_flag(broken + 4) != 0; }
   // its arrays one after the other, starting with array 0: row `row` of the array at `from`
   __device__ __forceinline__ RowView view(const T* from, int64_t stride, uint32_t row, bool landed) {
     RowView v;
@@ -265,12 +288,10 @@ struct Ring {
     }
     return v;
   }
-  // before the walker's memory is left
-  __device__ __forceinline__ void finish() {
-    if (threadIdx.x == 0 && is_broken()) {
-      const uint32_t rows = put_row - first_row;
-      for (uint32_t r = rows > static_cast<uint32_t>(rows_ahead) ? rows - rows_ahead : 0; r < rows; ++r) (void)wait_for(full + r % rows_ahead * 8, r / rows_ahead & 1u);
-    }
+  // Behind the last row: nothing is in flight, unless it was the one whose wait ran out.
+  __device__ __forceinline__ void finish() const {
+    const uint32_t rows = last_row - first_row;
+    if (rows > 0 && read_flag(broken) == rows) (void)wait_for(full + (rows - 1) % rows_ahead * 8, (rows - 1) / rows_ahead & 1u, kSpinLimit);
   }
 };
 

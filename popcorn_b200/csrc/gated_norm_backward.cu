@@ -15,6 +15,8 @@
 // its end.  With several gate rows a walker also writes a line of k whenever the gate row
 // changes, at index walker + gate row, which no other pair (walker, gate row) has.  gated_columns_kernel adds the lines up
 // in a fixed order: the result does not depend on timing.
+#include <cstdlib>
+
 #include "gated_norm.cuh"
 
 namespace b200 {
@@ -38,21 +40,21 @@ struct BackwardArgs {
 
 template <typename T, bool VEC, int TPR, bool ROW_GATE>
 __global__ void __launch_bounds__(TPR, kMaxWalk / TPR)
-gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
+gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes, uint32_t probes) {
   using PW = Pairs<T, VEC>;
   constexpr int N = PW::N, P = PW::P, ITEMS = kColumns / N;
   const int cols = a.columns, words = (cols + N - 1) / N;
   const RowShape shape = {cols, a.pairs};
   extern __shared__ __align__(128) unsigned char memory[];
   __shared__ uint64_t barriers[kMaxSlots];
-  __shared__ int flag;
+  __shared__ uint32_t flags[2];
   __shared__ float sums_store[2][4][16];
   pdl_prologue();
   const int lane_in_row = threadIdx.x, walker = blockIdx.x;
   const uint32_t first = range_start(a.rows, a.walkers, walker), last = range_start(a.rows, a.walkers, walker + 1);
   Ring<T, VEC, TPR> ring;
   const bool has_gs = a.gs != nullptr;
-  ring.start(barriers, memory, &flag, slots, static_cast<uint32_t>(cols) * sizeof(T), slot_bytes, first, last, 3 + (ROW_GATE ? 1 : 0) + (has_gs ? 1 : 0),
+  ring.start(barriers, memory, flags, slots, static_cast<uint32_t>(cols) * sizeof(T), slot_bytes, first, last, 3 + (ROW_GATE ? 1 : 0) + (has_gs ? 1 : 0),
              [&](int array, const T*& base, int64_t& ld) {
                base = array == 0 ? a.x : array == 1 ? a.residual : array == 2 ? a.gy : ROW_GATE && array == 3 ? a.gate : a.gs;
                ld = array == 0 ? a.ldx : array == 1 ? a.ldr : array == 2 ? a.ldgy : ROW_GATE && array == 3 ? a.ldgate : a.ldgs;
@@ -129,9 +131,10 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
       gate_end += a.period;
       load_factor(gate_row);
     }
-    const float r1 = stat.x, r2 = stat.y;
+    float r1 = stat.x, r2 = stat.y;
     if (row + 1 < last) stat = a.stats[row + 1];
-    const bool landed = ring.wait();
+    const bool landed = ring.wait(row - first, probes, TPR == 32 || tight);
+    if (!landed && ring.unsound()) r1 = r2 = NAN;
     const RowView xv = ring.view(a.x, a.ldx, row, landed), rv = ring.view(a.residual, a.ldr, row, landed), gyv = ring.view(a.gy, a.ldgy, row, landed);
     const RowView gv = ROW_GATE ? ring.view(a.gate, a.ldgate, row, landed) : gyv, gsv = has_gs ? ring.view(a.gs, a.ldgs, row, landed) : gyv;
     const Float2x r12 = both(r1), r22 = both(r2);
@@ -170,7 +173,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
     for (int n = 0; n < 4; ++n) sums[n] = pair_total(acc[n]);
     row_sums<TPR>(sums, sums_store[parity]);
     // every thread of the walker is past the row before: its slots can be filled again
-    if (TPR > 32 && !tight) ring.release(row - first);
+    if (TPR > 32 && !tight) ring.release(row - first, row - first);
     const float c2 = r2 * r2 * r2 * (sums[0] * a.inv_cols);
     // sums 1 to 3 hold r1 f x, and grad_x takes r1 x: c1 = r1^2 (r1 <f ds, x>) / cols, c1 x = (c1 / r1) r1 x
     const float inner = sums[1] + r2 * sums[2] - c2 * sums[3];
@@ -213,7 +216,7 @@ gated_backward_kernel(const BackwardArgs<T> a, int slots, uint32_t slot_bytes) {
     }
     if (TPR == 32 || tight) {
       __syncthreads();
-      ring.release(row - first + 1);
+      ring.release(row - first, row - first + 1);
     }
   }
   ring.finish();
@@ -379,11 +382,18 @@ BackwardPlan plan_backward(int64_t rows, int64_t cols, int64_t gate_rows, size_t
   return p;
 }
 
+// B200_GATED_WAIT_PROBES=<n> in the environment replaces the limit of a wait for a row's copies (read at every call; with 0 every
+// row is fetched with ordinary loads).
+uint32_t wait_probes() {
+  const char* v = std::getenv("B200_GATED_WAIT_PROBES");
+  return v != nullptr ? static_cast<uint32_t>(std::strtoul(v, nullptr, 10)) : kSpinLimit;
+}
+
 template <typename T, bool VEC, int TPR, bool ROW_GATE>
 int launch_backward(const BackwardArgs<T>& a, const WalkPlan& p, cudaStream_t st) {
   constexpr auto kernel = gated_backward_kernel<T, VEC, TPR, ROW_GATE>;
   if (int rc = allow_smem<kernel, kRingBytes>("gated_backward_kernel")) return rc;
-  launch(kernel, static_cast<unsigned>(p.walkers), TPR, static_cast<size_t>(p.slots) * p.slot_bytes, st, a, p.slots, p.slot_bytes);
+  launch(kernel, static_cast<unsigned>(p.walkers), TPR, static_cast<size_t>(p.slots) * p.slot_bytes, st, a, p.slots, p.slot_bytes, wait_probes());
   return after_launch("gated_backward_kernel");
 }
 

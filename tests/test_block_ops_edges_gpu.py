@@ -1,8 +1,12 @@
 """Calls at the edges of the operators around the layers: gates and logits that are no ordinary numbers, calls from several threads,
 derivatives that the kernels do not have."""
 
+import os
+import subprocess
+import sys
 import threading
 import time
+from pathlib import Path
 
 import pytest
 import torch
@@ -113,3 +117,36 @@ def test_rms_norm_gradients_of_several_widths_from_several_threads():
                     lambda: torch.equal(grad_x, want[0]) and torch.equal(grad_w, want[1]))
         return make
     assert not errors_from_threads([width_of(hidden) for hidden in (6144, 6144, 6144, 6144, 4160)], 1.5)
+
+
+def backwards_whose_waits_run_out():
+    """Run in a process of its own: the library counts such waits, and elsewhere there are none."""
+    before = 0
+    for rows, hidden, dtype, post, gate, with_gs in (
+            (12000, 256, BF16, True, "channel", True), (9000, 1000, BF16, True, "row", True), (3001, 4096, BF16, True, "row", True), (3001, 4096, F16, False, None, False),
+            (1000, 5120, F16, True, "first", True), (700, 8192, F32, True, "row", True), (700, 8192, F32, True, "channel", True), (700, 8192, BF16, True, "first", False),
+            (1, 4096, BF16, True, "channel", True), (2000, 2050, F32, True, "row", True), (2000, 2049, BF16, True, "channel", True), (9000, 515, F32, False, "first", True)):
+        lead = (rows // 100, 100) if gate == "first" else (rows,)
+        inputs = norm_inputs(hidden, lead, hidden, dtype, post, gate)
+        gy, gs = normal(5, *lead, hidden, dtype=dtype), normal(6, *lead, hidden, dtype=dtype) if with_gs else None
+        stats = ops.gated_add_rms_norm_forward(*inputs, "tanh")[2]
+        want = ops.gated_add_rms_norm_backward(gy, gs, *inputs, stats, "tanh")
+        torch.cuda.synchronize()
+        assert _lib.wait_timeouts() == before
+        for probes in (0, 1, 3):
+            os.environ["B200_GATED_WAIT_PROBES"] = str(probes)
+            for _ in range(3):
+                got = ops.gated_add_rms_norm_backward(gy, gs, *inputs, stats, "tanh")
+                for have, wanted in zip(got, want):
+                    assert have is wanted is None or torch.equal(have, wanted), (rows, hidden, dtype, gate, probes)
+            now = _lib.wait_timeouts()
+            assert probes > 0 or now > before
+            before = now
+        del os.environ["B200_GATED_WAIT_PROBES"]
+
+
+def test_norm_backward_whose_waits_run_out():
+    """Rows that are not there when their wait ends are fetched without the ring: the same bits, and the count of such waits goes up."""
+    child = subprocess.run([sys.executable, "-c", "from tests.test_block_ops_edges_gpu import backwards_whose_waits_run_out as run; run()"], cwd=Path(__file__).resolve().parents[1],
+                           capture_output=True, text=True, timeout=300)
+    assert child.returncode == 0, child.stderr[-2000:]
