@@ -311,6 +311,28 @@ class _AddRmsNorm(torch.autograd.Function):
         return grad_x, grad_x, grad_w, None, None
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """Gradients of a backward kernel while autograd records the backward pass (create_graph): to differentiate them raises, instead
+    of leaving their share out.  Takes the number of gradients, them, and the tensors that they are functions of."""
+
+    @staticmethod
+    def forward(ctx, name: str, count: int, *tensors: Tensor):
+        ctx.name = name
+        return tensors[:count]
+
+    @staticmethod
+    def backward(ctx, *_grads):
+        raise RuntimeError(f"{ctx.name} has no second derivative")
+
+
+def _first_order(name: str, grads: tuple[Tensor | None, ...], *depends: Tensor | None) -> tuple[Tensor | None, ...]:
+    if not torch.is_grad_enabled():
+        return grads
+    given = [g for g in grads if g is not None]
+    marked = iter(_NoSecondDerivative.apply(name, len(given), *given, *(t for t in depends if t is not None)))
+    return tuple(None if g is None else next(marked) for g in grads)
+
+
 class _GatedAddRmsNorm(torch.autograd.Function):
     """Saves the inputs and two numbers per row; the backward forms s again from x and residual, in fp32."""
 
@@ -331,6 +353,7 @@ class _GatedAddRmsNorm(torch.autograd.Function):
         if grad_y is None:  # only the residual stream was used downstream
             grad_y = torch.zeros_like(grad_s)
         grads = ops.gated_add_rms_norm_backward(grad_y, grad_s, x, residual, weight, post_weight, gate, stats, *ctx.options)
+        grads = _first_order("gated_add_rms_norm", grads, grad_y, grad_s, x, residual, weight, post_weight, gate)
         return (*grads, None, None, None, None, None)
 
 
@@ -349,7 +372,8 @@ class _MoeBalanceLoss(torch.autograd.Function):
         router_logits, mask, stats, table = ctx.saved_tensors
         if grad_balance is None and grad_z is None:
             return None, None, None, None
-        return ops.moe_balance_loss_backward(grad_balance, grad_z, router_logits, mask, stats, table, ctx.per_sequence), None, None, None
+        grad = ops.moe_balance_loss_backward(grad_balance, grad_z, router_logits, mask, stats, table, ctx.per_sequence)
+        return *_first_order("moe_balance_loss", (grad,), grad_balance, grad_z, router_logits), None, None, None
 
 
 class _Embedding(torch.autograd.Function):
@@ -362,7 +386,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_out: Tensor):
         (ids,) = ctx.saved_tensors
-        return None, ops.embedding_backward(grad_out, ids, *ctx.options), None, None
+        return None, *_first_order("embedding", (ops.embedding_backward(grad_out, ids, *ctx.options),), grad_out), None, None
 
 
 def rms_norm(x: Tensor, weight: Tensor, bias: Tensor | None = None, eps: float = 1e-6) -> Tensor:

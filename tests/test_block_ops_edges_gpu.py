@@ -11,8 +11,8 @@ from pathlib import Path
 import pytest
 import torch
 
-from popcorn_b200 import _lib, ops
-from tests.test_block_ops_gpu import BF16, DEV, F16, F32, check_norm, near, norm_inputs, norm_reference, normal
+from popcorn_b200 import _lib, autograd, ops
+from tests.test_block_ops_gpu import BF16, DEV, F16, F32, check_norm, ids_of, near, norm_inputs, norm_reference, normal, picks_of
 
 pytestmark = pytest.mark.gpu
 
@@ -150,3 +150,22 @@ def test_norm_backward_whose_waits_run_out():
     child = subprocess.run([sys.executable, "-c", "from tests.test_block_ops_edges_gpu import backwards_whose_waits_run_out as run; run()"], cwd=Path(__file__).resolve().parents[1],
                            capture_output=True, text=True, timeout=300)
     assert child.returncode == 0, child.stderr[-2000:]
+
+
+def test_second_derivatives_are_refused():
+    """A gradient penalty would otherwise go without these operators' share; first derivatives of a recorded backward stay as they are."""
+    x, residual, weight, post, gate = (t.requires_grad_(True) for t in norm_inputs(1, (6,), 64, F32, True, "channel"))
+    logits = normal(2, 20, 8).requires_grad_(True)
+    table = normal(3, 30, 16).requires_grad_(True)
+    picks, ids = picks_of(logits.detach(), 2), ids_of("zipf", 20, 30, 4).to(DEV)
+    for leaf, value in ((x, lambda: autograd.gated_add_rms_norm(x, residual, weight, post, gate)[0].sum()), (gate, lambda: autograd.gated_add_rms_norm(x, residual, weight, post, gate)[1].square().sum()),
+                        (logits, lambda: autograd.moe_balance_loss(logits, picks)[0]), (table, lambda: autograd.embedding(ids, table).square().sum())):
+        (plain,) = torch.autograd.grad(value(), leaf)
+        (recorded,) = torch.autograd.grad(value(), leaf, create_graph=True)
+        assert torch.equal(plain, recorded)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.grad(recorded.square().sum() + leaf.square().sum(), leaf)
+    # the gradient of a table does not depend on the table
+    (recorded,) = torch.autograd.grad(autograd.embedding(ids, table).sum(), table, create_graph=True)
+    (got,) = torch.autograd.grad(recorded.sum() + table.square().sum(), table)
+    assert torch.equal(got, 2 * table.detach())
