@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from popcorn_b200 import ops
 
@@ -486,11 +487,13 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int 
 
 
 def _needs_grad(*tensors: Tensor | None) -> bool:
+    """Whether autograd has to see the call: a tensor wants a gradient, or carries a tangent of forward mode (which the functions
+    refuse; past them it would be lost)."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return False
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def moe_grouped_gemm(rows: Tensor, weight: Tensor, offsets: Tensor, up_weight: Tensor | None = None) -> Tensor:

@@ -2,7 +2,10 @@
 
 import ctypes
 
-from popcorn_b200 import _lib
+import torch
+from torch.autograd import forward_ad
+
+from popcorn_b200 import _lib, autograd
 from tests.test_block_ops import FAKE, NULL, refused
 
 
@@ -14,3 +17,13 @@ def test_embedding_tables_whose_row_counter_would_wrap_are_refused(built_library
         assert refused("b200_embedding_backward_scratch_bytes", 4, vocab, 1, ctypes.byref(need)) == "B200_ERR_SHAPE"
         assert refused("b200_embedding", FAKE, FAKE, FAKE, 4, vocab, 1, 1, 1, 1, _lib.BF16, 1.0, NULL) == "B200_ERR_SHAPE"
         assert refused("b200_embedding_backward", FAKE, FAKE, FAKE, 4, vocab, 1, 1, -1, 1, _lib.BF16, 1.0, FAKE, ctypes.c_size_t(1 << 40), NULL) == "B200_ERR_SHAPE"
+
+
+def test_a_tangent_counts_as_a_gradient():
+    x = torch.ones(3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        for enabled in (True, False):
+            with torch.set_grad_enabled(enabled):
+                assert autograd._needs_grad(None, x, dual) and not autograd._needs_grad(x, None)
+    assert not autograd._needs_grad(x) and autograd._needs_grad(x.requires_grad_(True))

@@ -10,6 +10,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from popcorn_b200 import _lib, autograd, ops
 from tests.test_block_ops_gpu import BF16, DEV, F16, F32, check_norm, ids_of, near, norm_inputs, norm_reference, normal, picks_of
@@ -169,3 +170,18 @@ def test_second_derivatives_are_refused():
     (recorded,) = torch.autograd.grad(autograd.embedding(ids, table).sum(), table, create_graph=True)
     (got,) = torch.autograd.grad(recorded.sum() + table.square().sum(), table)
     assert torch.equal(got, 2 * table.detach())
+
+
+def test_forward_mode_is_refused():
+    x, residual, weight, post, gate = norm_inputs(1, (6,), 64, BF16, True, "channel")
+    logits, table, ids = normal(2, 20, 8), normal(3, 30, 16), ids_of("zipf", 20, 30, 4).to(DEV)
+    picks = picks_of(logits, 2)
+    rows, offsets, experts = normal(4, 32, 64, dtype=BF16), torch.tensor([0, 16, 32], dtype=torch.int32, device=DEV), normal(5, 2, 64, 64, dtype=BF16)
+    calls = ((x, lambda t: autograd.gated_add_rms_norm(t, residual, weight, post, gate)), (gate, lambda t: autograd.gated_add_rms_norm(x, residual, weight, post, t)),
+             (logits, lambda t: autograd.moe_balance_loss(t, picks)), (table, lambda t: autograd.embedding(ids, t)), (experts, lambda t: autograd.moe_grouped_gemm(rows, t, offsets)))
+    for enabled in (True, False):
+        with torch.set_grad_enabled(enabled), forward_ad.dual_level():
+            for tensor, call in calls:
+                call(tensor)
+                with pytest.raises(RuntimeError):
+                    call(forward_ad.make_dual(tensor, torch.ones_like(tensor)))
