@@ -185,3 +185,59 @@ def test_forward_mode_is_refused():
                 call(tensor)
                 with pytest.raises(RuntimeError):
                     call(forward_ad.make_dual(tensor, torch.ones_like(tensor)))
+
+
+@pytest.mark.parametrize("per_sequence", [False, True])
+@pytest.mark.parametrize("experts,dtype", [(64, F32), (64, BF16), (61, F32), (8, F16), (512, F32)])
+def test_balance_values_with_experts_switched_off(experts, dtype, per_sequence):
+    """Experts at -inf or at the type's lowest value have no share at all; the losses and the other experts' gradients are held to
+    bounds that those logits do not enter."""
+    logits = normal(4, 4, 50, experts, dtype=dtype)
+    off = torch.zeros(4, 50, experts, dtype=torch.bool, device=DEV)
+    off[..., 5] = True
+    off[:, ::3, experts // 4: experts // 2] = True
+    lowest = torch.zeros_like(off)
+    lowest[:, ::3, experts // 4: experts // 2] = True
+    off[1, 7, 1:] = True  # one expert is left
+    logits[off] = float("-inf")
+    logits[lowest & (normal(6, 4, 50, experts) > 0)] = torch.finfo(dtype).min
+    indices = picks_of(logits, 2)
+    weights = (0.3, 0.02)
+    leaf = logits.detach().requires_grad_(True)
+    balance, z, counts = autograd.moe_balance_loss(leaf, indices, None, per_sequence)
+    (grad,) = torch.autograd.grad((balance, z), leaf, tuple(torch.tensor(w, device=DEV) for w in weights))
+    groups = [slice(b, b + 1) for b in range(4)] if per_sequence else [slice(0, 4)]
+    wide = logits.double().masked_fill(off, float("-inf"))
+    p, lse = torch.softmax(wide, -1), torch.logsumexp(wide, -1, keepdim=True)
+    # exp of a difference of logits is off by roundings of the largest difference that counts; the rest as in the plain test
+    top = wide.amax(-1, keepdim=True)
+    size = 1 + torch.where(off, 0.0, top - wide).amax(-1, keepdim=True)
+    gb, gz = (float(torch.tensor(w)) for w in weights)
+    want_b, want_grad, bound = 0.0, torch.zeros_like(wide), torch.zeros_like(wide)
+    for g in groups:
+        picked = torch.bincount(indices[g].reshape(-1).long(), minlength=experts)
+        n = logits[g].shape[0] * 50
+        f = picked.double() * experts / (2 * n)
+        want_b = want_b + (f * p[g].reshape(-1, experts).mean(0)).sum() / len(groups)
+        inner = (p[g] * f).sum(-1, keepdim=True)
+        want_grad[g] = p[g] * (gb / (len(groups) * n) * (f - inner) + 2 * gz / 200 * lse[g])
+        bound[g] = p[g] * (gb / (len(groups) * n) * (f + inner) + 2 * gz / 200 * (lse[g].abs() + top[g].abs() + 1)) * size[g]
+        assert torch.equal((counts[g.start] if per_sequence else counts).long(), picked)
+    near(balance.detach(), want_b, want_b * float(size.max()), what="balance")
+    near(z.detach(), lse.square().mean(), (lse.abs() + top.abs() + 1).square().mean(), what="z")
+    near(grad, want_grad, bound, what="grad")
+    assert not grad[off].any()
+    # and each tolerance is far below the value that it is for
+    assert float(size.max()) < 50 and float((lse.abs() + top.abs() + 1).square().mean()) < 50 * float(lse.square().mean())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_expanded_rows_go_through_the_plain_ops(dtype):
+    """Rows that overlap in memory (stride 0) are copied first: the values of the contiguous call."""
+    row, other, weight = normal(1, 64, dtype=dtype), normal(2, 5, 64, dtype=dtype), normal(3, 64, dtype=dtype)
+    x = row.expand(5, 64)
+    for call in (lambda t: (ops.rms_norm(t, weight),), lambda t: ops.add_rms_norm(t, other, weight), lambda t: (ops.swiglu(t, other),), lambda t: (ops.layer_norm(t, weight),),
+                 lambda t: ops.rms_norm_backward(other, t, weight)[:2], lambda t: ops.swiglu_backward(t, other, other), lambda t: ops.moe_route(t, 4)):
+        for have, want in zip(call(x), call(x.contiguous())):
+            assert torch.equal(have, want)
+    assert torch.equal(x, row.expand(5, 64)) and x.stride(0) == 0
