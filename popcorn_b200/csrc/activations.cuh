@@ -17,7 +17,8 @@ namespace b200 {
 //          the full 32768 x 14336 bf16 configuration bit-identical to MATH 0
 //          and to the PyTorch CPU reference (the rounding of silu to bf16
 //          hides the last-bit fp32 differences).
-// 16-bit dtypes use MATH 1; fp32, whose results are not rounded again, uses MATH 0.
+// 16-bit dtypes use MATH 1; fp32, whose results are not rounded again, uses MATH 0 (except for a row's own gate in the gated
+// norm's backward, see activate_row).
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

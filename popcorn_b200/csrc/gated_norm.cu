@@ -128,14 +128,14 @@ gated_add_rms_wide_kernel(const ForwardArgs<T> a, int64_t cols) {
   float sum = 0.f;
   for (int64_t c = threadIdx.x; c < cols; c += 512) {
     const float f = branch_factor(a.post, gr, c, a.offset, a.scale, a.act);
-    const float s = stream_value<T>(Num<T>::up(xr[c]), Num<T>::up(rr[c]), f, r1, a.residual_scale);
+    const float s = stream_value(Num<T>::up(xr[c]), Num<T>::up(rr[c]), f, r1, a.residual_scale);
     sum = __fmaf_rn(s, s, sum);
   }
   const float r2 = inv_rms(row_sum<512>(sum, slots[1]), a.inv_cols, a.eps);
   if (a.stats != nullptr && threadIdx.x == 0) a.stats[row] = make_float2(r1, r2);
   for (int64_t c = threadIdx.x; c < cols; c += 512) {
     const float f = branch_factor(a.post, gr, c, a.offset, a.scale, a.act);
-    const float s = stream_value<T>(Num<T>::up(xr[c]), Num<T>::up(rr[c]), f, r1, a.residual_scale);
+    const float s = stream_value(Num<T>::up(xr[c]), Num<T>::up(rr[c]), f, r1, a.residual_scale);
     a.s[row * a.lds + c] = Num<T>::down(s);
     a.y[row * a.ldy + c] = Num<T>::down(s * r2 * (Num<T>::up(a.weight[c]) + a.offset));
   }

@@ -78,7 +78,7 @@ __device__ __forceinline__ float activation_slope(float value, int act) {
 // 1 / sqrt(sum of squares / cols + eps), within two units in the last place (nothing is rounded to T in between)
 __device__ __forceinline__ float inv_rms(float sumsq, float inv_cols, float eps) { return rsqrtf(fmaf(sumsq, inv_cols, eps)); }
 
-// N sums over the TPR threads of a row, TPR a power of two.  Up to a warp: shuffles.  Wider: one barrier
+// A sum over the TPR threads of a row, TPR a power of two.  Up to a warp: shuffles.  Wider: one barrier
 // (rows wider than a warp have the CTA to themselves); `slot` is shared memory that no thread still reads from an earlier
 // call.
 template <int TPR>
@@ -423,7 +423,6 @@ constexpr int kWalkColumns = kMaxWalk * kColumns;
 constexpr int kRingBytes = 196 * 1024;  // of an SM; the rest of its 228 KB is what 16 CTAs need besides
 
 // s of one element, for the kernels that go over a row more than once
-template <typename T>
 __device__ __forceinline__ float stream_value(float x, float residual, float factor, float r1, float residual_scale) {
   return fmaf(r1 * factor, x, residual_scale * residual);
 }

@@ -258,7 +258,7 @@ gated_backward_wide_kernel(const BackwardArgs<T> a, int64_t cols, bool row_gate)
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
     for (int64_t c = threadIdx.x; c < cols; c += kBackwardThreads) {
       const float f = branch_factor(a.post, gr, c, a.offset, a.scale, a.act), x = Num<T>::up(xr[c]);
-      const float s = stream_value<T>(x, Num<T>::up(rr[c]), f, r1, a.residual_scale);
+      const float s = stream_value(x, Num<T>::up(rr[c]), f, r1, a.residual_scale);
       const float gw = Num<T>::up(gyr[c]) * (Num<T>::up(a.weight[c]) + a.offset), u = f * x;
       sums[0] = fmaf(gw, s, sums[0]);
       if (gsr != nullptr) sums[1] = fmaf(u, Num<T>::up(gsr[c]), sums[1]);
@@ -273,7 +273,7 @@ gated_backward_wide_kernel(const BackwardArgs<T> a, int64_t cols, bool row_gate)
       const float p = a.post == nullptr ? 1.f : Num<T>::up(a.post[c]) + a.offset;
       const float value = gr == nullptr ? 1.f : activate<T>(Num<T>::up(gr[c]), a.act);
       const float branch = a.scale * value, f = branch * p, x = Num<T>::up(xr[c]), gy = Num<T>::up(gyr[c]);
-      const float s = stream_value<T>(x, Num<T>::up(rr[c]), f, r1, a.residual_scale);
+      const float s = stream_value(x, Num<T>::up(rr[c]), f, r1, a.residual_scale);
       const float ds = fmaf(-c2, s, fmaf(r2, gy * (Num<T>::up(a.weight[c]) + a.offset), gsr == nullptr ? 0.f : Num<T>::up(gsr[c])));
       const float k = ds * x * r1;
       a.dx[row * a.ldo + c] = Num<T>::down(fmaf(r1 * f, ds, -c1 * x));
